@@ -251,8 +251,8 @@ def prepare(case, seed):
         samq = _samq()
         s["handle"] = samq.Weights(TYPES[case["weights"]], k, gguf.shape[0], gguf.cpu().numpy())
         if op == "grouped":
-            s["workspace"] = _workspace(samq.linear_grouped_workspace(
-                s["handle"], case["experts"], rows, s["x"].dtype, gathered=s["row_index"] is not None))
+            s["workspace"] = _workspace(samq.linear_grouped_workspace(s["handle"], case["experts"], s["x"].shape[0], rows,
+                                                                      s["x"].dtype))
         else:
             s["adapters"] = samq.Adapters(k, n, case["rank"], case["adapters"])
             a, b, scale = s["a"].cpu().numpy(), s["b"].cpu().numpy(), s["scale"].tolist()
@@ -316,8 +316,10 @@ def _stage(x):
         return x.float()
     v = x.view(x.shape[0], -1, 32)
     amax = v.abs().amax(-1, keepdim=True)
-    d = (amax / 127).half().float()
-    t = v.abs() * torch.where(amax == 0, torch.zeros_like(amax), 127 / amax)
+    # quotients of two tensors: torch turns one by or of a Python number into a product with a rounded reciprocal
+    top = torch.full_like(amax, 127)
+    d = (amax / top).half().float()
+    t = v.abs() * torch.where(amax == 0, torch.zeros_like(amax), top / amax)
     whole = t.trunc()
     q = torch.copysign(whole + (t - whole >= 0.5), v)
     return (d * q).half().float().view(x.shape)
@@ -468,8 +470,8 @@ def _operand64(x):
         return x.double()
     blocks = x.reshape(-1, 32)
     peak = blocks.abs().max(1, keepdim=True).values
-    step = (peak / 127).half().double()
-    scaled = blocks * torch.where(peak > 0, 127 / peak, peak)
+    step = (peak.double() / 127).float().half().double()
+    scaled = blocks * torch.where(peak > 0, (127 / peak.double()).float(), peak)
     code = torch.floor(scaled.double().abs() + 0.5) * torch.sign(scaled.double())
     return (step * code).half().double().reshape(x.shape)
 
