@@ -556,6 +556,103 @@ typedef struct samq_neck_v1 {
 samq_status samq_neck_forward_v1(const samq_neck_v1* neck, const float* x, int grid_w, int grid_h,
                                  float* const out[4], void* stream);
 
+/* ---- Routed linears ------------------------------------------------------------
+ * Linears whose weight depends on the row, beside samq_linear_v1: the products
+ * of a mixture of experts (GGML's mul_mat over a stacked [k, n, experts] tensor
+ * by row ids) with the router's plan before and the weighted sum after them,
+ * and low-rank adapters of many requests over one shared projection.
+ *
+ * Types: x_type and y_type are SAMQ_TYPE_F16 or SAMQ_TYPE_F32, independently.
+ * f32 activations are staged by the Q8_1 rule of samq_stage_f16_v1 (into the
+ * workspace), f16 activations are the operand itself, as in
+ * samq_linear_f16_v1.  The weight operand is the decoded packed weight rounded
+ * to f16 whatever the row count; products accumulate in f32; f16 outputs are
+ * rounded once (values beyond f16's range become infinities).
+ *
+ * These calls keep no memory of the library between them: what they need is
+ * the caller's workspace, of at least the size the ..._workspace_v1 call
+ * states for the same arguments (16-byte aligned; NULL where it states 0).
+ * Calls that may overlap in time need workspaces of their own.  They
+ * allocate nothing and may be captured into a graph once samq_init_v1 (or a
+ * handle's creation) has run on the device.  Index arrays (offsets, row_index,
+ * rows, slots, ids) are device int32; values out of range never reach memory
+ * out of range (the rules are stated with each). */
+
+/* The router: for each of `tokens` rows of device f32 logits [tokens][ld]
+ * (ld >= experts), the top_k experts of largest logit, ties to the lower
+ * index.  A logit that is not finite is not eligible (a masked expert is
+ * -INFINITY); a token with fewer than top_k eligible experts leaves its other
+ * choices empty: id -1, weight 0, slot -1.  1 <= top_k <= min(32, experts),
+ * experts <= 1024, tokens <= 2^20.
+ *   weights [tokens][top_k]: exp(logit - max) / sum, the sum over the chosen
+ *     experts (normalize != 0) or over all eligible ones (normalize == 0);
+ *   ids     [tokens][top_k]: the experts in order of falling logit;
+ *   offsets [experts + 1]: expert e owns the plan rows offsets[e] ..
+ *     offsets[e + 1] - 1 (the `offsets` of samq_linear_grouped_v1);
+ *   rows    [tokens * top_k]: the token of each plan row, the rows of an
+ *     expert in order of (token, choice); -1 from offsets[experts] on;
+ *   slots   [tokens][top_k]: the plan row of each choice (the inverse). */
+size_t samq_route_workspace_v1(int64_t tokens, int experts, int top_k);
+samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int64_t ld, int top_k, int normalize,
+                          float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Grouped product: w holds `groups` stacked matrices ([groups * n][k] GGUF
+ * rows, n = rows of w / groups, any n).  For every group g and every row i of
+ * offsets[g] .. offsets[g + 1] - 1
+ *   y[i] = act(W_g x[row_index ? row_index[i] : i] + bias[g]),
+ * x [x_rows][ldx], y [rows][ldy], bias [groups][n] or NULL, offsets
+ * [groups + 1] non-decreasing within [0, rows], row_index [rows] or NULL
+ * (then x_rows >= rows).  Rows of y outside every group are left as they
+ * were; a row_index outside [0, x_rows) stands for a row of zeros; offsets
+ * are clamped to [0, rows].  ldx and ldy are multiples of 4 (f32) or 8 (f16)
+ * elements, x and y 16-byte aligned; y overlaps no input.  groups <= 1024,
+ * rows and x_rows <= 2^24. */
+size_t samq_linear_grouped_workspace_v1(const samq_weights* weights, int groups, int64_t x_rows, int64_t rows,
+                                        int x_type);
+samq_status samq_linear_grouped_v1(const samq_weights* weights, int groups, const void* x, int x_type, int64_t x_rows,
+                                   int64_t ldx, const int32_t* row_index, const int32_t* offsets, int64_t rows,
+                                   const float* bias, int epilogue, void* y, int y_type, int64_t ldy, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* The weighted sum back: out[t] = residual[t] + sum over j < top_k of
+ * weights[t][j] * y[slots[t][j]] in order of j, accumulated in f32.  y
+ * [y_rows][ldy] of y_type; a slot outside [0, y_rows) adds nothing (its
+ * weight is not read as a factor); residual f32 [tokens][ldr] or NULL (zero),
+ * may be out itself; out f32 [tokens][ldo].  width % 4 == 0 (f32 y) or
+ * % 8 == 0 (f16 y), strides likewise, pointers 16-byte aligned, top_k <= 32. */
+samq_status samq_combine_v1(const void* y, int y_type, int64_t y_rows, int64_t ldy, const int32_t* slots,
+                            const float* weights, int64_t tokens, int top_k, int64_t width, const float* residual,
+                            int64_t ldr, float* out, int64_t ldo, void* stream);
+
+/* A set of `count` adapter slots for a projection of shape k -> n: slot a
+ * holds A_a [rank][k], B_a [n][rank] (as f16) and a scale.  1 <= max_rank <=
+ * 128, 1 <= count <= 4096.  Slots start empty (they add nothing). */
+typedef struct samq_adapters samq_adapters;
+samq_status samq_adapters_create_v1(int device, int64_t k, int64_t n, int max_rank, int count, void* stream,
+                                    samq_adapters** out);
+/* Fills a slot from HOST arrays a [rank][k] and b [n][rank] of `type` F32
+ * (rounded to f16) or F16; rank 0 empties it.  Every value must be finite in
+ * f16 (else SAMQ_ERR_PAYLOAD, the slot unchanged).  Ordered on `stream` after
+ * the calls already there and complete on return; calls on other streams that
+ * use the slot must have finished. */
+samq_status samq_adapters_set_v1(samq_adapters* adapters, int slot, int rank, const void* a, const void* b, int type,
+                                 float scale, void* stream);
+samq_status samq_adapters_destroy_v1(samq_adapters* adapters);
+
+/* The shared projection with every row's own adapter:
+ *   y[i] = act(W x[i] + bias + scale_a B_a (A_a x[i])), a = ids[i],
+ * for m rows; an ids[i] outside [0, count) is a row without adapter.
+ * scale_a A_a x[i] is kept to f32's precision as a pair of f16 values and
+ * must lie within the f16 operand range (else SAMQ_ERR_RANGE from
+ * samq_check_v1).  m <= 2^24; strides, alignment and types as above. */
+size_t samq_linear_adapters_workspace_v1(const samq_weights* weights, const samq_adapters* adapters, int64_t m,
+                                         int x_type);
+samq_status samq_linear_adapters_v1(const samq_weights* weights, const samq_adapters* adapters, const void* x,
+                                    int x_type, int64_t m, int64_t ldx, const int32_t* ids, const float* bias,
+                                    int epilogue, void* y, int y_type, int64_t ldy, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* Counters of a handle.  Mirrors ggml_cuda_sam_q8_rhs_query_v1
  * (cmake/patches/ggml-native-activation.patch:34-42). */
 samq_status samq_query_v1(const samq_weights* weights, struct samq_counters_v1* out);

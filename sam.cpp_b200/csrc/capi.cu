@@ -235,6 +235,21 @@ void release_dense(samq_dense* w) {
     delete w;
 }
 
+void release_adapters(samq_adapters* w) {
+    if (!w) return;
+    if (w->device >= 0) {
+        int previous = -1;
+        cudaGetDevice(&previous);
+        cudaSetDevice(w->device);
+        if (w->a) cudaFree(w->a);
+        if (w->b2) cudaFree(w->b2);
+        if (w->scale) cudaFree(w->scale);
+        if (w->ranks) cudaFree(w->ranks);
+        if (previous >= 0) cudaSetDevice(previous);
+    }
+    delete w;
+}
+
 void release(samq_weights* w) {
     if (!w) return;
     if (w->device >= 0) {
@@ -1192,6 +1207,281 @@ samq_status samq_neck_forward_v1(const samq_neck_v1* neck, const float* x, int g
         cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
         Scratch& scratch = scratch_for(state, stream, neck_scratch_bytes(*neck, grid_w, grid_h));
         launch_neck(*neck, x, grid_w, grid_h, out, scratch.ptr, state, stream);
+    });
+}
+
+// ---- routed linears ---------------------------------------------------------
+
+namespace {
+
+constexpr int64_t kMaxRoutedRows = int64_t(1) << 24;
+constexpr int kMaxGroups = 1024;
+constexpr int kMaxTopK = 32;
+constexpr int kMaxAdapterRank = 128;
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+void check_element_type(int type, const char* message) {
+    require(type == SAMQ_TYPE_F32 || type == SAMQ_TYPE_F16, message);
+}
+
+void check_rows(const void* p, int type, int64_t width, int64_t ld, const char* message) {
+    require(p != nullptr && aligned16(p) && ld >= width && ld % (type == SAMQ_TYPE_F16 ? 8 : 4) == 0 &&
+                ld <= (int64_t(1) << 32),
+            message);
+}
+
+void check_workspace(const void* workspace, size_t bytes, size_t needed) {
+    require(bytes >= needed, "workspace is smaller than the call needs");
+    require(needed == 0 || (workspace != nullptr && aligned16(workspace)), "workspace must be 16-byte aligned");
+}
+
+// The f16 operand of f32 activations in the workspace, on a 256-byte boundary.
+size_t staged_bytes(int64_t rows, int64_t k, int x_type) {
+    return x_type == SAMQ_TYPE_F32 ? (static_cast<size_t>(rows * k) * sizeof(__half) + 255) / 256 * 256 : 0;
+}
+
+// x as the product's operand: itself (f16) or staged into `staged` (f32).
+void routed_operand(RoutedProduct& p, const void* x, int x_type, int64_t x_rows, int64_t ldx, void* staged,
+                    DeviceState& state, cudaStream_t stream) {
+    p.x_rows = x_rows;
+    if (x_type == SAMQ_TYPE_F16) {
+        p.x = static_cast<const __half*>(x);
+        p.ldx = ldx;
+        return;
+    }
+    launch_act_f16(static_cast<const float*>(x), x_rows, p.k, ldx, static_cast<__half*>(staged), nullptr, state.status,
+                   stream);
+    p.x = static_cast<const __half*>(staged);
+    p.ldx = p.k;
+}
+
+RoutedProduct routed_product(const samq_weights* w, int groups, int64_t rows, const float* bias, int epilogue, void* y,
+                             int y_type, int64_t ldy) {
+    RoutedProduct p;
+    p.rows = rows;
+    p.groups = groups;
+    p.type = w->type;
+    p.packets = static_cast<const uint8_t*>(w->packets);
+    p.operand = w->operand;
+    p.k = static_cast<int>(w->k);
+    p.n = static_cast<int>(w->n / groups);
+    p.bias = bias;
+    p.gelu = epilogue == SAMQ_EPILOGUE_GELU_ERF ? 1 : 0;
+    p.y = y;
+    p.y_type = y_type;
+    p.ldy = ldy;
+    return p;
+}
+
+// IEEE binary16 of `count` host values; false if one is not finite there.
+bool host_f16(const void* src, int type, size_t count, __half* dst) {
+    for (size_t i = 0; i < count; ++i) {
+        dst[i] = type == SAMQ_TYPE_F16 ? static_cast<const __half*>(src)[i]
+                                       : __float2half_rn(static_cast<const float*>(src)[i]);
+        if ((__half_as_ushort(dst[i]) & 0x7c00u) == 0x7c00u) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+size_t samq_route_workspace_v1(int64_t tokens, int experts, int top_k) {
+    if (tokens < 0 || experts <= 0 || top_k <= 0) return 0;
+    return route_workspace_bytes(tokens, experts, top_k);
+}
+
+samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int64_t ld, int top_k, int normalize,
+                          float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots,
+                          void* workspace, size_t workspace_bytes, void* stream_ptr) {
+    return guarded([&] {
+        require(tokens >= 0 && tokens <= (int64_t(1) << 20), "token count out of range");
+        require(experts >= 1 && experts <= kMaxGroups, "expert count out of range");
+        require(top_k >= 1 && top_k <= kMaxTopK && top_k <= experts, "top_k must lie in [1, min(32, experts)]");
+        require(ld >= experts && ld <= (int64_t(1) << 32), "logit row stride must be >= experts");
+        require(offsets != nullptr && aligned4(offsets), "offsets must be a device int32 pointer");
+        const void* arrays[] = {logits, weights, ids, rows, slots};
+        for (const void* a : arrays) require(tokens == 0 || (a != nullptr && aligned4(a)), "null or misaligned array");
+        check_workspace(workspace, workspace_bytes, samq_route_workspace_v1(tokens, experts, top_k));
+        DeviceState& state = device_state(current_device());
+        launch_route(logits, tokens, experts, ld, top_k, normalize, weights, ids, offsets, rows, slots, workspace,
+                     state, static_cast<cudaStream_t>(stream_ptr));
+    });
+}
+
+size_t samq_linear_grouped_workspace_v1(const samq_weights* w, int groups, int64_t x_rows, int64_t rows, int x_type) {
+    if (!w || groups <= 0 || x_rows < 0 || rows <= 0) return 0;
+    return staged_bytes(x_rows, w->k, x_type);
+}
+
+samq_status samq_linear_grouped_v1(const samq_weights* w, int groups, const void* x, int x_type, int64_t x_rows,
+                                   int64_t ldx, const int32_t* row_index, const int32_t* offsets, int64_t rows,
+                                   const float* bias, int epilogue, void* y, int y_type, int64_t ldy, void* workspace,
+                                   size_t workspace_bytes, void* stream_ptr) {
+    return guarded([&] {
+        require(w != nullptr, "null weights");
+        require(groups >= 1 && groups <= kMaxGroups && w->n % groups == 0,
+                "groups must lie in [1, 1024] and divide the weight rows");
+        check_element_type(x_type, "x_type must be F32 or F16");
+        check_element_type(y_type, "y_type must be F32 or F16");
+        require(rows >= 0 && rows <= kMaxRoutedRows && x_rows >= 0 && x_rows <= kMaxRoutedRows, "row count out of range");
+        require(epilogue == SAMQ_EPILOGUE_NONE || epilogue == SAMQ_EPILOGUE_GELU_ERF, "unknown epilogue");
+        require(row_index != nullptr || x_rows >= rows, "x has fewer rows than the plan and no row_index is given");
+        if (rows == 0) return;
+        require(x_rows > 0, "x has no rows");
+        require(offsets != nullptr && aligned4(offsets) && aligned4(row_index) && aligned4(bias),
+                "offsets must be a device int32 pointer, row_index and bias 4-byte aligned");
+        check_rows(x, x_type, w->k, ldx, "x must be 16-byte aligned with a row stride >= k of whole 16-byte units");
+        check_rows(y, y_type, w->n / groups, ldy,
+                   "y must be 16-byte aligned with a row stride >= n of whole 16-byte units");
+        check_workspace(workspace, workspace_bytes,
+                        samq_linear_grouped_workspace_v1(w, groups, x_rows, rows, x_type));
+        DeviceGuard guard(w->device);
+        DeviceState& state = device_state(w->device);
+        cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+        RoutedProduct p = routed_product(w, groups, rows, bias, epilogue, y, y_type, ldy);
+        p.row_index = row_index;
+        p.offsets = offsets;
+        routed_operand(p, x, x_type, x_rows, ldx, workspace, state, stream);
+        launch_routed(p, state, stream);
+        const_cast<samq_weights*>(w)->launches.fetch_add(1);
+    });
+}
+
+samq_status samq_combine_v1(const void* y, int y_type, int64_t y_rows, int64_t ldy, const int32_t* slots,
+                            const float* weights, int64_t tokens, int top_k, int64_t width, const float* residual,
+                            int64_t ldr, float* out, int64_t ldo, void* stream_ptr) {
+    return guarded([&] {
+        check_element_type(y_type, "y_type must be F32 or F16");
+        require(tokens >= 0 && tokens <= kMaxRoutedRows && y_rows >= 0 && y_rows <= (int64_t(1) << 31) - 1,
+                "row count out of range");
+        require(top_k >= 1 && top_k <= kMaxTopK, "top_k must lie in [1, 32]");
+        require(width > 0 && width <= (int64_t(1) << 20) && width % (y_type == SAMQ_TYPE_F16 ? 8 : 4) == 0,
+                "width must be a positive multiple of 8 (f16) or 4 (f32)");
+        if (tokens == 0) return;
+        require(slots != nullptr && weights != nullptr && aligned4(slots) && aligned4(weights),
+                "slots and weights must be device pointers");
+        if (y_rows > 0)
+            check_rows(y, y_type, width, ldy, "y must be 16-byte aligned with a row stride >= width of whole 16-byte units");
+        check_rows(out, SAMQ_TYPE_F32, width, ldo, "out must be 16-byte aligned with a row stride >= width, a multiple of 4");
+        if (residual)
+            check_rows(residual, SAMQ_TYPE_F32, width, ldr,
+                       "residual must be 16-byte aligned with a row stride >= width, a multiple of 4");
+        DeviceState& state = device_state(current_device());
+        launch_combine(y, y_type, y_rows, ldy, slots, weights, tokens, top_k, width, residual, ldr, out, ldo, state,
+                       static_cast<cudaStream_t>(stream_ptr));
+    });
+}
+
+samq_status samq_adapters_create_v1(int device, int64_t k, int64_t n, int max_rank, int count, void* stream_ptr,
+                                    samq_adapters** out) {
+    return guarded([&] {
+        require(out != nullptr, "null output handle");
+        *out = nullptr;
+        require(k > 0 && k % 32 == 0 && k <= (int64_t(1) << 20), "width must be a positive multiple of 32");
+        require(n > 0 && n <= (int64_t(1) << 24), "row count out of range");
+        require(max_rank >= 1 && max_rank <= kMaxAdapterRank, "max_rank must lie in [1, 128]");
+        require(count >= 1 && count <= 4096, "slot count must lie in [1, 4096]");
+        require(n * count <= (int64_t(1) << 30), "adapter set too large");
+        DeviceState& state = device_state(device);
+        (void)state;
+        DeviceGuard guard(device);
+        cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+        std::unique_ptr<samq_adapters, void (*)(samq_adapters*)> w(new samq_adapters, release_adapters);
+        w->device = device;
+        w->k = k;
+        w->n = n;
+        w->max_rank = max_rank;
+        w->rank = (max_rank + 15) / 16 * 16;
+        w->count = count;
+        const size_t a_bytes = static_cast<size_t>(count) * w->rank * k * sizeof(__half);
+        const size_t b_bytes = static_cast<size_t>(count) * n * 2 * w->rank * sizeof(__half);
+        check_cuda(cudaMalloc(reinterpret_cast<void**>(&w->a), a_bytes), "cudaMalloc(adapter A)");
+        check_cuda(cudaMalloc(reinterpret_cast<void**>(&w->b2), b_bytes), "cudaMalloc(adapter B)");
+        check_cuda(cudaMalloc(reinterpret_cast<void**>(&w->scale), count * sizeof(float)), "cudaMalloc(adapter scale)");
+        check_cuda(cudaMalloc(reinterpret_cast<void**>(&w->ranks), count * sizeof(int)), "cudaMalloc(adapter ranks)");
+        check_cuda(cudaMemsetAsync(w->a, 0, a_bytes, stream), "cudaMemsetAsync(adapter A)");
+        check_cuda(cudaMemsetAsync(w->b2, 0, b_bytes, stream), "cudaMemsetAsync(adapter B)");
+        check_cuda(cudaMemsetAsync(w->scale, 0, count * sizeof(float), stream), "cudaMemsetAsync(adapter scale)");
+        check_cuda(cudaMemsetAsync(w->ranks, 0, count * sizeof(int), stream), "cudaMemsetAsync(adapter ranks)");
+        check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize(adapters)");
+        *out = w.release();
+    });
+}
+
+samq_status samq_adapters_set_v1(samq_adapters* ad, int slot, int rank, const void* a, const void* b, int type,
+                                 float scale, void* stream_ptr) {
+    return guarded([&] {
+        require(ad != nullptr, "null adapters");
+        require(slot >= 0 && slot < ad->count, "slot out of range");
+        require(rank >= 0 && rank <= ad->max_rank, "rank must lie in [0, max_rank]");
+        check_element_type(type, "adapter type must be F32 or F16");
+        require(rank == 0 || (a != nullptr && b != nullptr), "null adapter array");
+        const size_t R = static_cast<size_t>(ad->rank), r = static_cast<size_t>(rank), k = static_cast<size_t>(ad->k),
+                     n = static_cast<size_t>(ad->n);
+        std::vector<__half> ha(R * k), rows(n * r), hb(n * 2 * R);  // zero beyond the rank
+        const float s = rank > 0 ? scale : 0.0f;
+        if (!(s - s == 0.0f) || !host_f16(a, type, r * k, ha.data()) || !host_f16(b, type, n * r, rows.data()))
+            fail(SAMQ_ERR_PAYLOAD, "adapter has a value that is not finite in f16, or a non-finite scale");
+        for (size_t j = 0; j < n; ++j)
+            for (size_t i = 0; i < r; ++i) hb[j * 2 * R + i] = hb[j * 2 * R + R + i] = rows[j * r + i];
+        DeviceGuard guard(ad->device);
+        cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+        const size_t at = static_cast<size_t>(slot);
+        check_cuda(cudaMemcpyAsync(ad->a + at * R * k, ha.data(), ha.size() * sizeof(__half), cudaMemcpyHostToDevice,
+                                   stream), "cudaMemcpyAsync(adapter A)");
+        check_cuda(cudaMemcpyAsync(ad->b2 + at * n * 2 * R, hb.data(), hb.size() * sizeof(__half),
+                                   cudaMemcpyHostToDevice, stream), "cudaMemcpyAsync(adapter B)");
+        check_cuda(cudaMemcpyAsync(ad->scale + at, &s, sizeof(s), cudaMemcpyHostToDevice, stream),
+                   "cudaMemcpyAsync(adapter scale)");
+        check_cuda(cudaMemcpyAsync(ad->ranks + at, &rank, sizeof(rank), cudaMemcpyHostToDevice, stream),
+                   "cudaMemcpyAsync(adapter rank)");
+        check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize(adapter)");
+    });
+}
+
+samq_status samq_adapters_destroy_v1(samq_adapters* adapters) {
+    return guarded([&] { release_adapters(adapters); });
+}
+
+size_t samq_linear_adapters_workspace_v1(const samq_weights* w, const samq_adapters* ad, int64_t m, int x_type) {
+    if (!w || !ad || m <= 0) return 0;
+    return staged_bytes(m, w->k, x_type) + static_cast<size_t>(m) * 2 * ad->rank * sizeof(__half);
+}
+
+samq_status samq_linear_adapters_v1(const samq_weights* w, const samq_adapters* ad, const void* x, int x_type,
+                                    int64_t m, int64_t ldx, const int32_t* ids, const float* bias, int epilogue,
+                                    void* y, int y_type, int64_t ldy, void* workspace, size_t workspace_bytes,
+                                    void* stream_ptr) {
+    return guarded([&] {
+        require(w != nullptr, "null weights");
+        require(ad != nullptr, "null adapters");
+        require(ad->k == w->k && ad->n == w->n, "the adapters are of another shape than the weights");
+        require(ad->device == w->device, "the adapters belong to another device than the weights");
+        check_element_type(x_type, "x_type must be F32 or F16");
+        check_element_type(y_type, "y_type must be F32 or F16");
+        require(m >= 0 && m <= kMaxRoutedRows, "row count out of range");
+        require(epilogue == SAMQ_EPILOGUE_NONE || epilogue == SAMQ_EPILOGUE_GELU_ERF, "unknown epilogue");
+        if (m == 0) return;
+        require(ids != nullptr && aligned4(ids) && aligned4(bias),
+                "ids must be a device int32 pointer, bias 4-byte aligned");
+        check_rows(x, x_type, w->k, ldx, "x must be 16-byte aligned with a row stride >= k of whole 16-byte units");
+        check_rows(y, y_type, w->n, ldy, "y must be 16-byte aligned with a row stride >= n of whole 16-byte units");
+        check_workspace(workspace, workspace_bytes, samq_linear_adapters_workspace_v1(w, ad, m, x_type));
+        DeviceGuard guard(w->device);
+        DeviceState& state = device_state(w->device);
+        cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+        RoutedProduct p = routed_product(w, 1, m, bias, epilogue, y, y_type, ldy);
+        routed_operand(p, x, x_type, m, ldx, workspace, state, stream);
+        __half* h2 = reinterpret_cast<__half*>(static_cast<uint8_t*>(workspace) + staged_bytes(m, w->k, x_type));
+        p.ids = ids;
+        p.h2 = h2;
+        p.b2 = ad->b2;
+        p.rank = ad->rank;
+        p.adapter_count = ad->count;
+        launch_adapter_down(p, *ad, h2, state, stream);
+        launch_routed(p, state, stream);
+        const_cast<samq_weights*>(w)->launches.fetch_add(1);
     });
 }
 

@@ -165,6 +165,18 @@ struct samq_mmq_weights {
     float* scales = nullptr;
 };
 
+// Low-rank adapters of one projection (k -> n), `count` slots of `rank` rows
+// (the largest rank rounded up to 16; unused rows are zero).
+struct samq_adapters {
+    int device = -1;
+    int64_t k = 0, n = 0;
+    int max_rank = 0, rank = 0, count = 0;
+    __half* a = nullptr;     // [count][rank][k]
+    __half* b2 = nullptr;    // [count][n][2 * rank]: B | B, against the hi | lo pair of the down product
+    float* scale = nullptr;  // [count]
+    int* ranks = nullptr;    // [count], 0: empty slot
+};
+
 // ---- launchers implemented in the .cu files -------------------------------
 namespace samq {
 
@@ -399,5 +411,42 @@ void launch_dense_gemm(const float* a_hi, const float* a_lo, const samq_dense& w
 size_t neck_scratch_bytes(const samq_neck_v1& neck, int grid_w, int grid_h);
 void launch_neck(const samq_neck_v1& neck, const float* x, int grid_w, int grid_h, float* const out[4], void* scratch,
                  DeviceState& state, cudaStream_t stream);
+
+
+// route.cu: the router's plan and the weighted sum of the routed linears.
+size_t route_workspace_bytes(int64_t tokens, int experts, int top_k);
+void launch_route(const float* logits, int64_t tokens, int experts, int64_t ld, int top_k, int normalize,
+                  float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace,
+                  DeviceState& state, cudaStream_t stream);
+void launch_combine(const void* y, int y_type, int64_t y_rows, int64_t ldy, const int32_t* slots, const float* weights,
+                    int64_t tokens, int top_k, int64_t width, const float* residual, int64_t ldr, float* out,
+                    int64_t ldo, DeviceState& state, cudaStream_t stream);
+
+// grouped.cu: products whose weight depends on the row.
+struct RoutedProduct {
+    const __half* x = nullptr;          // f16 operand [x_rows][ldx]
+    int64_t x_rows = 0, ldx = 0;
+    const int* row_index = nullptr;     // [rows] or null: row i of x
+    const int* offsets = nullptr;       // [groups + 1], or null: one group of all rows
+    int64_t rows = 0;
+    int groups = 1;
+    int type = 0;                       // of the packed weights
+    const uint8_t* packets = nullptr;   // K4 packets of the groups * n stacked rows
+    const __half* operand = nullptr;    // their f16 expansion
+    int k = 0, n = 0;                   // n: rows of one group
+    const float* bias = nullptr;        // [groups][n] or null
+    int gelu = 0;
+    void* y = nullptr;
+    int y_type = 0;
+    int64_t ldy = 0;
+    // Adapters (one group): slot ids, the hi | lo pair of scale_a A_a x and B | B.
+    const int* ids = nullptr;           // [rows] or null: no adapters
+    const __half* h2 = nullptr;         // [rows][2 * rank]
+    const __half* b2 = nullptr;         // [adapter_count][n][2 * rank]
+    int rank = 0, adapter_count = 0;
+};
+void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
+                         cudaStream_t stream);
+void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
 
 }  // namespace samq

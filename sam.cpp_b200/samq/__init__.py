@@ -183,6 +183,18 @@ SIGNATURES = {
     "samq_conv2d_v1": (_i32, [_vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp]),
     "samq_maxpool2x2_v1": (_i32, [_vp, _i32, _i32, _i64, _vp, _vp]),
     "samq_neck_forward_v1": (_i32, [ctypes.POINTER(NeckDesc), _vp, _i32, _i32, ctypes.POINTER(_vp), _vp]),
+    "samq_route_workspace_v1": (_sz, [_i64, _i32, _i32]),
+    "samq_route_v1": (_i32, [_vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "samq_linear_grouped_workspace_v1": (_sz, [_vp, _i32, _i64, _i64, _i32]),
+    "samq_linear_grouped_v1": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _i64,
+                                      _vp, _sz, _vp]),
+    "samq_combine_v1": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "samq_adapters_create_v1": (_i32, [_i32, _i64, _i64, _i32, _i32, _vp, ctypes.POINTER(_vp)]),
+    "samq_adapters_set_v1": (_i32, [_vp, _i32, _i32, _vp, _vp, _i32, ctypes.c_float, _vp]),
+    "samq_adapters_destroy_v1": (_i32, [_vp]),
+    "samq_linear_adapters_workspace_v1": (_sz, [_vp, _vp, _i64, _i32]),
+    "samq_linear_adapters_v1": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i32, _i64, _vp, _sz,
+                                       _vp]),
 }
 STATIC_OPERAND_ELEMENTS = 16777216
 
@@ -680,3 +692,161 @@ def neck_forward(neck: Neck, x, grid_w: int, grid_h: int, outs, stream=None):
     """samq_neck_forward_v1: the four NHWC feature maps of the ViT output x."""
     arr = (_vp * 4)(*[_addr(o) for o in outs])
     _check(library().samq_neck_forward_v1(ctypes.byref(neck.desc), _addr(x), grid_w, grid_h, arr, _stream(stream)))
+
+
+# ---- routed linears ----------------------------------------------------------
+# Element types come from the torch tensors (float16 or float32); index tensors
+# are int32 on the device.  `workspace` is a uint8 tensor of at least the
+# ..._workspace() size, kept by a caller that calls often or captures a graph;
+# without one a call that needs memory takes it from torch's caching allocator.
+
+def _element(dtype) -> int:
+    """F16 / F32 of a torch dtype (or the id itself)."""
+    if isinstance(dtype, int):
+        return dtype
+    name = str(dtype)
+    if name == "torch.float16":
+        return F16
+    if name == "torch.float32":
+        return F32
+    raise TypeError(f"float16 or float32 expected, got {name}")
+
+
+def _same_device(device: int | None, *tensors) -> int:
+    """The one device of the given tensors (None entries skipped), which must be `device` where that is given."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != "cuda" or (device is not None and t.device.index != device):
+            raise ValueError(f"tensor on {t.device}, expected cuda:{'' if device is None else device}")
+        device = t.device.index
+    return device
+
+
+def _int32(*tensors):
+    for t in tensors:
+        if t is not None and str(t.dtype) != "torch.int32":
+            raise TypeError(f"index tensors are int32, got {t.dtype}")
+
+
+def _stream_on(stream, device: int):
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _scratch(workspace, needed: int, device: int):
+    """(tensor kept alive by the caller, address, bytes) of a workspace."""
+    if workspace is None and needed:
+        import torch
+        workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
+    if workspace is None:
+        return None, None, 0
+    _same_device(device, workspace)
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def route_workspace(tokens: int, experts: int, top_k: int) -> int:
+    return library().samq_route_workspace_v1(tokens, experts, top_k)
+
+
+def route(logits, tokens: int, experts: int, ld: int, top_k: int, weights, ids, offsets, rows, slots,
+          normalize: bool = True, workspace=None, stream=None):
+    """samq_route_v1: the top_k experts of every row of logits, their weights and the plan sorted by expert."""
+    import torch
+    device = _same_device(None, logits, weights, ids, offsets, rows, slots)
+    _int32(ids, offsets, rows, slots)
+    if logits.dtype != torch.float32 or weights.dtype != torch.float32:
+        raise TypeError("logits and weights are float32")
+    keep, address, size = _scratch(workspace, 0 if workspace is not None else route_workspace(tokens, experts, top_k),
+                                   device)
+    with torch.cuda.device(device):
+        _check(library().samq_route_v1(logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0,
+                                       weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
+                                       slots.data_ptr(), address, size, _stream_on(stream, device)))
+
+
+def linear_grouped_workspace(w: Weights, groups: int, x_rows: int, rows: int, x_dtype) -> int:
+    return library().samq_linear_grouped_workspace_v1(w.handle, groups, x_rows, rows, _element(x_dtype))
+
+
+def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, rows: int, y, ldy: int, row_index=None,
+                   bias=None, epilogue: int = EPILOGUE_NONE, workspace=None, stream=None):
+    """samq_linear_grouped_v1: y[i] = act(W_g x[row_index[i]] + bias_g) for the rows offsets[g] .. offsets[g + 1] of
+    group g; w holds the groups' matrices stacked (w.n = groups * n)."""
+    device = _same_device(w.device, x, offsets, y, row_index, bias)
+    _int32(offsets, row_index)
+    xt, yt = _element(x.dtype), _element(y.dtype)
+    needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt)
+    keep, address, size = _scratch(workspace, needed, device)
+    _check(library().samq_linear_grouped_v1(w.handle, groups, x.data_ptr(), xt, x_rows, ldx, _addr(row_index),
+                                            offsets.data_ptr(), rows, _addr(bias), epilogue, y.data_ptr(), yt, ldy,
+                                            address, size, _stream_on(stream, device)))
+
+
+def combine(y, y_rows: int, ldy: int, slots, weights, tokens: int, top_k: int, width: int, out, ldo: int,
+            residual=None, ldr: int = 0, stream=None):
+    """samq_combine_v1: out[t] = residual[t] + sum_j weights[t][j] y[slots[t][j]]."""
+    import torch
+    device = _same_device(None, y, slots, weights, out, residual)
+    _int32(slots)
+    if any(t is not None and t.dtype != torch.float32 for t in (weights, out, residual)):
+        raise TypeError("weights, residual and out are float32")
+    with torch.cuda.device(device):
+        _check(library().samq_combine_v1(y.data_ptr(), _element(y.dtype), y_rows, ldy, slots.data_ptr(),
+                                         weights.data_ptr(), tokens, top_k, width, _addr(residual), ldr,
+                                         out.data_ptr(), ldo, _stream_on(stream, device)))
+
+
+class Adapters:
+    """Slots of low-rank adapters for a projection k -> n (samq_adapters*)."""
+
+    def __init__(self, k: int, n: int, max_rank: int, count: int, device: int = 0, stream=None):
+        handle = ctypes.c_void_p()
+        self.handle = None
+        _check(library().samq_adapters_create_v1(device, k, n, max_rank, count, _stream(stream), ctypes.byref(handle)))
+        self.handle = handle
+        self.k, self.n, self.max_rank, self.count, self.device = k, n, max_rank, count, device
+
+    def set(self, slot: int, a: np.ndarray, b: np.ndarray, scale: float, stream=None):
+        """Fills a slot from host arrays a [rank][k] and b [n][rank] (float32 or float16)."""
+        if a.dtype != b.dtype or a.dtype not in (np.float32, np.float16):
+            raise TypeError("a and b are both float32 or both float16")
+        if a.ndim != 2 or b.ndim != 2 or a.shape[1] != self.k or b.shape != (self.n, a.shape[0]):
+            raise ValueError("a is [rank][k], b is [n][rank]")
+        a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
+        _check(library().samq_adapters_set_v1(self.handle, slot, a.shape[0], a.ctypes.data, b.ctypes.data,
+                                              F16 if a.dtype == np.float16 else F32, scale, _stream(stream)))
+
+    def clear(self, slot: int, stream=None):
+        _check(library().samq_adapters_set_v1(self.handle, slot, 0, None, None, F16, 0.0, _stream(stream)))
+
+    def close(self):
+        if self.handle:
+            _check(library().samq_adapters_destroy_v1(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def linear_adapters_workspace(w: Weights, adapters: Adapters, m: int, x_dtype) -> int:
+    return library().samq_linear_adapters_workspace_v1(w.handle, adapters.handle, m, _element(x_dtype))
+
+
+def linear_adapters(w: Weights, adapters: Adapters, x, m: int, ldx: int, ids, y, ldy: int, bias=None,
+                    epilogue: int = EPILOGUE_NONE, workspace=None, stream=None):
+    """samq_linear_adapters_v1: y[i] = act(W x[i] + bias + scale_a B_a (A_a x[i])) with a = ids[i] (none if out of
+    range)."""
+    device = _same_device(w.device, x, ids, y, bias)
+    _int32(ids)
+    xt, yt = _element(x.dtype), _element(y.dtype)
+    needed = 0 if workspace is not None else linear_adapters_workspace(w, adapters, m, xt)
+    keep, address, size = _scratch(workspace, needed, device)
+    _check(library().samq_linear_adapters_v1(w.handle, adapters.handle, x.data_ptr(), xt, m, ldx, ids.data_ptr(),
+                                             _addr(bias), epilogue, y.data_ptr(), yt, ldy, address, size,
+                                             _stream_on(stream, device)))
