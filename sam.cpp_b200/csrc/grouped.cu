@@ -125,6 +125,10 @@ void launch_adapter_down(const RoutedProduct& p, const samq_adapters& ad, __half
 }
 
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream) {
+    if (p.rows > 64) {
+        launch_routed_tile(p, 1, state, stream);
+        return;
+    }
     const int64_t tiles = std::min<int64_t>(p.rows, p.rows / kTile + p.groups);
     const dim3 grid(static_cast<unsigned>((p.n + kTile - 1) / kTile), static_cast<unsigned>(tiles));
     if (p.y_type == SAMQ_TYPE_F16)

@@ -1,0 +1,491 @@
+// routed_tile.cu -- the routed product for groups of many rows, on the tensor
+// cores: y[i] = act(W_g x[row_index[i]] + bias_g + delta_i) over tiles of 128 (or
+// 256, a CTA pair) consecutive plan rows of one group by BN weight rows.
+//
+// Mathematics.  One tile is D = X_tile . W_tile^T over k, in f32 in TMEM.  The
+// adapters ride on the same accumulator as more depth:
+//   delta_i = B_a h_i, h_i = scale_a A_a x_i (a = ids[i]),
+//   D += [hi(H) | lo(H)]_a . [B_a | B_a]^T for every adapter a with rows in the tile,
+// where row i of the left factor is h_i's f16 pair if ids[i] == a and zero
+// otherwise.  The zero rows cost nothing to make: the left factor is a TMA
+// gather by row index, and an index past the end reads zeros.  The pair keeps h
+// to 2^-22, f32's level against the f16 rounding of B.
+//
+// The same gather (tile::gather4, four rows an instruction, one per lane of the
+// producer warp) reads x by row_index, so no permuted copy of x is made.
+//
+// Pipeline (64 + 32 * kEpilogueWarps threads, one CTA or CTA pair per SM or TPC,
+// persistent over the tiles of all groups):
+//   warp 0     producer: 128 x 64 of X and BN (a pair: BN / 2 each) x 64 of W per
+//              step by TMA, 128-byte swizzle, kStages deep.  Each step's `last`
+//              flag travels with its stage, as only the producer knows how many
+//              adapters a tile has;
+//   warp 1     TMEM owner; one thread (of the even CTA) issues tcgen05.mma;
+//   warps 2..  epilogue: accumulator out of TMEM, bias, erf-GELU, stores of 32
+//              bytes a lane (a whole L2 sector) straight from registers, rows
+//              past the group's end left alone.  The next tile's MMAs overlap it.
+// Every wait is bounded.  No load uses multicast.
+#include <algorithm>
+
+#include "samq_internal.hpp"
+
+namespace samq {
+namespace {
+
+constexpr int BM = 128;  // rows of a CTA's tile
+constexpr int BK = 64;   // depth of a step: one 128-byte swizzle row of f16
+constexpr int kAccStride = 256;
+constexpr int kEpilogueWarps = 16;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kMaxGroups = 1024;
+constexpr int kSmemLimit = 232448;
+
+template <int CTAS, int BN>
+struct TileSmem {
+    static constexpr int a_bytes = BM * BK * 2;
+    static constexpr int b_bytes = BN / CTAS * BK * 2;
+    static constexpr int stage = a_bytes + b_bytes;
+    static constexpr int tables = 3 * (kMaxGroups + 1) * 4;  // tile prefix, begin, end of each group
+    static constexpr int fixed = 1024 + tables + 512;
+    static constexpr int stages = (kSmemLimit - fixed) / stage > 8 ? 8 : (kSmemLimit - fixed) / stage;
+    static constexpr int b_off = stages * a_bytes;
+    static constexpr int table_off = stages * stage;
+    static constexpr int bar_off = (table_off + tables + 15) / 16 * 16;
+    static constexpr int total = stages * stage + fixed;
+};
+
+struct TileMaps {
+    CUtensorMap x;       // box 64 x 128 rows (x in plan order)
+    CUtensorMap x_rows;  // box 64 x 1, gathered
+    CUtensorMap w;       // box 64 x BN / CTAS
+    CUtensorMap h;       // adapters: [rows][2 rank], box 64 x 1, gathered
+    CUtensorMap b;       // adapters: [adapters * n][2 rank], box 64 x BN / CTAS
+};
+
+// Four rows of 64 columns by index into shared memory (the map's box is one row
+// high).  CTAS == 2: `bar` is the shared::cluster address of either CTA's barrier.
+template <int CTAS>
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int x, int4 r) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+            "%4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+            "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+            : "memory");
+}
+
+template <int CTAS>
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* local, uint32_t bar, int x,
+                                         int y) {
+    if constexpr (CTAS == 1) tma_load_2d(dst, map, local, x, y);
+    else tma_load_2d_pair(dst, map, bar, x, y);
+}
+
+// 32 bytes of one row: a whole L2 sector where the row allows it.
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
+                     "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+        *(reinterpret_cast<uint4*>(dst) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+__device__ __forceinline__ int clamp_row(int v, int64_t rows) {
+    return v < 0 ? 0 : v > rows ? static_cast<int>(rows) : v;
+}
+
+struct Tile {
+    int group, row0, end, col0;  // plan rows row0 .. end - 1, columns col0 ..
+};
+
+// The groups' tiles in order: s_first[g] is the number of row tiles before group g.
+__device__ __forceinline__ Tile find_tile(int tile, int n_tiles, int bn, int rows_per_tile, int groups,
+                                          const int* s_first, const int* s_begin, const int* s_end) {
+    const int rt = tile / n_tiles;
+    int lo = 0, hi = groups;  // s_first[lo] <= rt < s_first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= rt) lo = mid;
+        else hi = mid;
+    }
+    Tile t;
+    t.group = lo;
+    t.row0 = s_begin[lo] + (rt - s_first[lo]) * rows_per_tile;
+    t.end = s_end[lo];
+    t.col0 = (tile - rt * n_tiles) * bn;
+    return t;
+}
+
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p, int min_rows, DeviceStatus* status) {
+    using L = TileSmem<CTAS, BN>;
+    constexpr int kStages = L::stages;
+    static_assert(kStages >= 3 && L::total <= kSmemLimit, "shared memory budget");
+    static_assert(2 * 8 * kStages + 5 * 8 + 8 + 4 * kStages <= 512, "barrier space");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sa = smem;
+    uint8_t* sb = smem + L::b_off;
+    int* s_first = reinterpret_cast<int*>(smem + L::table_off);
+    int* s_begin = s_first + kMaxGroups + 1;
+    int* s_end = s_begin + kMaxGroups + 1;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
+    uint64_t* empty = full + kStages;
+    uint64_t* tfull = empty + kStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* last_step = reinterpret_cast<int*>(tmem_slot + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CTAS == 2 ? static_cast<int>(cluster_cta_rank()) : 0;
+    const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
+    constexpr int kTileRows = CTAS * BM;
+    const int n_tiles = (p.n + BN - 1) / BN;
+    const int kblocks = (p.k + BK - 1) / BK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], CTAS * kEpilogueWarps);
+        }
+        mbar_init(drain, 1);
+        fence_barrier_init();
+        tma_prefetch_desc(&maps.x);
+        tma_prefetch_desc(&maps.w);
+    }
+    if (warp == 1) {
+        if constexpr (CTAS == 2) tmem_alloc_pair(tmem_slot, 2 * kAccStride);
+        else tmem_alloc(tmem_slot, 2 * kAccStride);
+    }
+    // What the previous kernel may write is read from here on.
+    pdl_wait();
+    if (warp == 2) {
+        int carry = 0;
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + lane;
+            int begin = 0, end = 0, tiles = 0;
+            if (g < p.groups) {
+                begin = p.offsets ? clamp_row(__ldg(p.offsets + g), p.rows) : 0;
+                end = p.offsets ? max(begin, clamp_row(__ldg(p.offsets + g + 1), p.rows)) : static_cast<int>(p.rows);
+                tiles = end - begin >= min_rows ? (end - begin + kTileRows - 1) / kTileRows : 0;
+                s_begin[g] = begin;
+                s_end[g] = end;
+            }
+            int sum = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            if (g < p.groups) s_first[g] = carry + sum - tiles;
+            carry += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) s_first[p.groups] = carry;
+    }
+    tc_fence_before();
+    if constexpr (CTAS == 2) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int tiles = s_first[p.groups] * n_tiles;
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        uint32_t issued = 0, issued_phase = 0;
+        bool ok = true;
+        const int nothing = static_cast<int>(p.x_rows), no_row = static_cast<int>(p.rows);  // indices that read zeros
+        // One step into the next stage: B from `bm`, A as a tile (am != null) or gathered by r from `gm`.
+        auto step = [&](const CUtensorMap* am, int arow, const CUtensorMap* gm, int4 r, const CUtensorMap* bm, int brow,
+                        int x, bool last) -> bool {
+            bool free = true;
+            if (lane == 0) free = mbar_wait(&empty[s], ph ^ 1u, status, 61);
+            if (!__shfl_sync(0xffffffffu, free, 0)) return false;
+            const uint32_t bar = CTAS == 2 ? cluster_map(&full[s], 0) : smem_u32(&full[s]);
+            if (lane == 0) {
+                if (rank == 0) {
+                    last_step[s] = last;
+                    mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
+                }
+                tma_tile<CTAS>(sb + s * L::b_bytes, bm, &full[s], bar, x, brow + rank * (BN / CTAS));
+                if (am) tma_tile<CTAS>(sa + s * L::a_bytes, am, &full[s], bar, x, arow);
+            }
+            __syncwarp();
+            if (!am) tma_gather4<CTAS>(sa + s * L::a_bytes + lane * 512, gm, bar, x, r);
+            issued |= 1u << s;
+            issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
+            if (++s == kStages) {
+                s = 0;
+                ph ^= 1u;
+            }
+            return true;
+        };
+        for (int tile = unit; tile < tiles && ok; tile += units) {
+            const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
+            const int row0 = t.row0 + rank * BM;
+            const int mine = row0 + 4 * lane;  // this lane's four rows of the CTA's 128
+            int4 src = make_int4(nothing, nothing, nothing, nothing);
+            if (p.row_index) {
+                int v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = mine + j < t.end ? __ldg(p.row_index + mine + j) : nothing;
+                    v[j] = r >= 0 && r < nothing ? r : nothing;
+                }
+                src = make_int4(v[0], v[1], v[2], v[3]);
+            }
+            // The pair's 256 rows hold the same adapters for both CTAs.
+            int own[4], other[4];
+            int next = p.adapter_count;
+            if (p.ids) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    own[j] = mine + j < t.end ? __ldg(p.ids + mine + j) : -1;
+                    const int o = CTAS == 2 ? (rank ? mine + j - BM : mine + j + BM) : mine + j;
+                    other[j] = o < t.end ? __ldg(p.ids + o) : -1;
+                    if (own[j] >= 0) next = min(next, own[j]);
+                    if (other[j] >= 0) next = min(next, other[j]);
+                }
+                next = __reduce_min_sync(0xffffffffu, next);
+            }
+            const int wrow = t.group * p.n + t.col0;
+            const CUtensorMap* am = p.row_index ? nullptr : &maps.x;
+            for (int kb = 0; kb < kblocks && ok; ++kb)
+                ok = step(am, row0, &maps.x_rows, src, &maps.w, wrow, kb * BK,
+                          kb == kblocks - 1 && next >= p.adapter_count);
+            while (ok && next < p.adapter_count) {
+                const int a = next;
+                next = p.adapter_count;
+                int v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = own[j] == a ? mine + j : no_row;
+                    if (own[j] > a) next = min(next, own[j]);
+                    if (other[j] > a) next = min(next, other[j]);
+                }
+                next = __reduce_min_sync(0xffffffffu, next);
+                const int4 rows4 = make_int4(v[0], v[1], v[2], v[3]);
+                for (int c = 0; c < 2 * p.rank && ok; c += BK)
+                    ok = step(nullptr, 0, &maps.h, rows4, &maps.b, a * p.n + t.col0, c,
+                              c + BK >= 2 * p.rank && next >= p.adapter_count);
+            }
+        }
+        pdl_trigger();  // all loads issued
+        if (!ok && lane == 0) {
+            // Let the copies in flight land before the CTA exits.
+            if constexpr (CTAS == 1) {
+                for (int i = 0; i < kStages; ++i)
+                    if (issued & (1u << i)) mbar_wait(&full[i], (issued_phase >> i) & 1u, status, 65);
+            } else {
+                const uint64_t start = global_timer_ns();
+                while (global_timer_ns() - start < 2000000ull) __nanosleep(1000);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_f16_f32(CTAS * BM, BN);
+            int s = 0;
+            uint32_t ph = 0;
+            int acc = 0;
+            uint32_t acc_ph = 0;
+            bool ok = true;
+            for (int tile = unit; tile < tiles && ok; tile += units) {
+                const bool free = CTAS == 2 ? mbar_wait_cluster(&tempty[acc], acc_ph ^ 1u, status, 62)
+                                            : mbar_wait(&tempty[acc], acc_ph ^ 1u, status, 62);
+                if (!free) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kAccStride);
+                bool first = true, last = false;
+                while (!last) {
+                    if (!mbar_wait(&full[s], ph, status, 63)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    last = last_step[s] != 0;
+                    const uint32_t a_addr = smem_u32(sa + s * L::a_bytes);
+                    const uint32_t b_addr = smem_u32(sb + s * L::b_bytes);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; ++kk) {
+                        const uint64_t ad = smem_desc_sw128(a_addr + kk * 32), bd = smem_desc_sw128(b_addr + kk * 32);
+                        if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad, bd, idesc, first ? 0u : 1u);
+                        else tc_mma_f16(d, ad, bd, idesc, first ? 0u : 1u);
+                        first = false;
+                    }
+                    if constexpr (CTAS == 2) {
+                        tc_commit_pair(cluster_map(&empty[s], 0));
+                        tc_commit_pair(cluster_map(&empty[s], 1));
+                    } else {
+                        tc_commit(&empty[s]);
+                    }
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if constexpr (CTAS == 2) {
+                    tc_commit_pair(cluster_map(&tfull[acc], 0));
+                    tc_commit_pair(cluster_map(&tfull[acc], 1));
+                } else {
+                    tc_commit(&tfull[acc]);
+                }
+                acc ^= 1;
+                if (acc == 0) acc_ph ^= 1u;
+            }
+            // Every MMA this thread issued is complete before TMEM is released.
+            if constexpr (CTAS == 2) tc_commit_pair(cluster_map(drain, 0));
+            else tc_commit(drain);
+            mbar_wait(drain, 0, status, 66);
+        }
+        __syncwarp();
+    } else {
+        constexpr int kParts = kEpilogueWarps / 4;
+        constexpr int kChunks = BN / 32;
+        const int quarter = warp & 3;      // TMEM lanes 32 * quarter ..
+        const int part = (warp - 2) >> 2;  // its share of the columns
+        const bool f16 = p.y_type == SAMQ_TYPE_F16;
+        const int elem = f16 ? 2 : 4;
+        const bool vec = p.ldy * elem % 16 == 0;
+        const bool wide = p.ldy * elem % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
+        int acc = 0;
+        uint32_t acc_ph = 0;
+        for (int tile = unit; tile < tiles; tile += units) {
+            const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
+            const int row = t.row0 + rank * BM + quarter * 32 + lane;
+            // Warp-uniform: the TMEM loads below are warp-collective.
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 64))) break;
+            tc_fence_after();
+            uint8_t* out = static_cast<uint8_t*>(p.y) + (static_cast<int64_t>(row) * p.ldy + t.col0) * elem;
+            const float* bias = p.bias ? p.bias + static_cast<int64_t>(t.group) * p.n + t.col0 : nullptr;
+#pragma unroll 1
+            for (int c = part * kChunks / kParts * 32; c < (part + 1) * kChunks / kParts * 32; c += 32) {
+                const int left = p.n - t.col0 - c;  // columns of this chunk inside the group
+                if (left <= 0) break;
+                const float bias_lane = bias && lane < left ? __ldg(bias + c + lane) : 0.0f;
+                uint32_t r[32];
+                tc_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                     static_cast<uint32_t>(acc * kAccStride + c),
+                                 r);
+                tc_wait_ld();
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + __shfl_sync(0xffffffffu, bias_lane, i);
+                if (p.gelu) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = gelu_erf(v[i]);
+                }
+                if (row < t.end) {
+                    if (left >= 32 && vec) {
+                        if (f16) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                uint32_t o[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const __half2 h = __floats2half2_rn(v[16 * j + 2 * i], v[16 * j + 2 * i + 1]);
+                                    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+                                }
+                                store32(out + c * 2 + 32 * j, o, wide);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t o[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[8 * j + i]);
+                                store32(out + c * 4 + 32 * j, o, wide);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i < left) {
+                                if (f16) reinterpret_cast<__half*>(out)[c + i] = __float2half_rn(v[i]);
+                                else reinterpret_cast<float*>(out)[c + i] = v[i];
+                            }
+                        }
+                    }
+                }
+                __syncwarp();  // converged for the next chunk's collective TMEM load
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CTAS == 2) mbar_arrive_cluster(cluster_map(&tempty[acc], 0));
+                else mbar_arrive(&tempty[acc]);
+            }
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1u;
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    // A pair: both CTAs are done with TMEM and with each other's barriers.
+    if constexpr (CTAS == 2) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, 2 * kAccStride);
+        else tmem_dealloc(tmem_base, 2 * kAccStride);
+    }
+}
+
+template <int CTAS, int BN>
+void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
+    using L = TileSmem<CTAS, BN>;
+    TileMaps maps;
+    const auto f16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
+    encode_tensor_map_2d(&maps.x, f16, p.x, p.k, p.x_rows, p.ldx * 2, BK, BM, sw);
+    encode_tensor_map_2d(&maps.x_rows, f16, p.x, p.k, p.x_rows, p.ldx * 2, BK, 1, sw);
+    encode_tensor_map_2d(&maps.w, f16, p.operand, p.k, static_cast<uint64_t>(p.groups) * p.n,
+                         static_cast<uint64_t>(p.k) * 2, BK, BN / CTAS, sw);
+    maps.h = maps.x_rows;
+    maps.b = maps.w;
+    if (p.ids) {
+        encode_tensor_map_2d(&maps.h, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, 1, sw);
+        encode_tensor_map_2d(&maps.b, f16, p.b2, 2 * p.rank, static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank,
+                             BK, BN / CTAS, sw);
+    }
+    auto kernel = routed_tile_kernel<CTAS, BN>;
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    set_smem_limit_once(state, fn, L::total, "cudaFuncSetAttribute(routed tile smem)");
+    const int64_t tiles = (p.rows / (CTAS * BM) + p.groups) * ((p.n + BN - 1) / BN);  // at most
+    if constexpr (CTAS == 2) {
+        const int resident =
+            pair_clusters_resident(state, fn, kThreads, L::total, "cudaOccupancyMaxActiveClusters(routed tile)");
+        const int64_t pairs = std::min<int64_t>(tiles, resident);
+        launch_pdl_pairs(kernel, dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), L::total, stream,
+                         "routed_tile_kernel launch", maps, p, min_rows, state.status);
+    } else {
+        const int64_t ctas = std::min<int64_t>(tiles, state.sm_count);
+        launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), L::total, stream,
+                   "routed_tile_kernel launch", maps, p, min_rows, state.status);
+    }
+}
+
+}  // namespace
+
+void launch_routed_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
+    if (p.rows >= 256 * p.groups) run_tile<2, 256>(p, min_rows, state, stream);
+    else run_tile<1, 128>(p, min_rows, state, stream);
+}
+
+}  // namespace samq

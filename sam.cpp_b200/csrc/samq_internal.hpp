@@ -448,5 +448,7 @@ struct RoutedProduct {
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
                          cudaStream_t stream);
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
+// routed_tile.cu: the groups of at least `min_rows` rows on tensor-core tiles.
+void launch_routed_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream);
 
 }  // namespace samq
