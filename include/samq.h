@@ -609,7 +609,7 @@ samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int6
  * elements, x and y 16-byte aligned; y overlaps no input.  groups <= 1024,
  * rows and x_rows <= 2^24. */
 size_t samq_linear_grouped_workspace_v1(const samq_weights* weights, int groups, int64_t x_rows, int64_t rows,
-                                        int x_type);
+                                        int x_type, int indexed /* a row_index is given */);
 samq_status samq_linear_grouped_v1(const samq_weights* weights, int groups, const void* x, int x_type, int64_t x_rows,
                                    int64_t ldx, const int32_t* row_index, const int32_t* offsets, int64_t rows,
                                    const float* bias, int epilogue, void* y, int y_type, int64_t ldy, void* workspace,

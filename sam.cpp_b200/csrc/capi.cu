@@ -1236,23 +1236,35 @@ void check_workspace(const void* workspace, size_t bytes, size_t needed) {
     require(needed == 0 || (workspace != nullptr && aligned16(workspace)), "workspace must be 16-byte aligned");
 }
 
-// The f16 operand of f32 activations in the workspace, on a 256-byte boundary.
-size_t staged_bytes(int64_t rows, int64_t k, int x_type) {
-    return x_type == SAMQ_TYPE_F32 ? (static_cast<size_t>(rows * k) * sizeof(__half) + 255) / 256 * 256 : 0;
+// Whether the product's operand is a copy in the workspace: f32 activations are
+// staged there, and rows taken by index are brought into plan order for the tile
+// kernel (which a call of few rows does not run).
+bool copies_operand(int x_type, int64_t rows, bool indexed) {
+    return x_type == SAMQ_TYPE_F32 || (indexed && rows > kRoutedFewRows);
 }
 
-// x as the product's operand: itself (f16) or staged into `staged` (f32).
-void routed_operand(RoutedProduct& p, const void* x, int x_type, int64_t x_rows, int64_t ldx, void* staged,
-                    DeviceState& state, cudaStream_t stream) {
-    p.x_rows = x_rows;
-    if (x_type == SAMQ_TYPE_F16) {
+// Its bytes, a multiple of 256.
+size_t operand_bytes(int64_t rows, int64_t k, bool copied) {
+    return copied ? (static_cast<size_t>(rows * k) * sizeof(__half) + 255) / 256 * 256 : 0;
+}
+
+// Fills in the operand of `p`: x itself or its copy at `copy`.
+void routed_operand(RoutedProduct& p, const void* x, int x_type, int64_t x_rows, int64_t ldx, const int32_t* row_index,
+                    void* copy, DeviceState& state, cudaStream_t stream) {
+    if (!copies_operand(x_type, p.rows, row_index != nullptr)) {
         p.x = static_cast<const __half*>(x);
+        p.x_rows = x_rows;
         p.ldx = ldx;
+        p.row_index = row_index;
         return;
     }
-    launch_act_f16(static_cast<const float*>(x), x_rows, p.k, ldx, static_cast<__half*>(staged), nullptr, state.status,
-                   stream);
-    p.x = static_cast<const __half*>(staged);
+    __half* out = static_cast<__half*>(copy);
+    if (row_index)
+        launch_gather_rows(x, x_type, x_rows, ldx, row_index, p.rows, p.k, out, state, stream);
+    else
+        launch_act_f16(static_cast<const float*>(x), p.rows, p.k, ldx, out, nullptr, state.status, stream);
+    p.x = out;
+    p.x_rows = p.rows;
     p.ldx = p.k;
 }
 
@@ -1309,9 +1321,10 @@ samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int6
     });
 }
 
-size_t samq_linear_grouped_workspace_v1(const samq_weights* w, int groups, int64_t x_rows, int64_t rows, int x_type) {
+size_t samq_linear_grouped_workspace_v1(const samq_weights* w, int groups, int64_t x_rows, int64_t rows, int x_type,
+                                        int indexed) {
     if (!w || groups <= 0 || x_rows < 0 || rows <= 0) return 0;
-    return staged_bytes(x_rows, w->k, x_type);
+    return operand_bytes(rows, w->k, copies_operand(x_type, rows, indexed != 0));
 }
 
 samq_status samq_linear_grouped_v1(const samq_weights* w, int groups, const void* x, int x_type, int64_t x_rows,
@@ -1335,14 +1348,13 @@ samq_status samq_linear_grouped_v1(const samq_weights* w, int groups, const void
         check_rows(y, y_type, w->n / groups, ldy,
                    "y must be 16-byte aligned with a row stride >= n of whole 16-byte units");
         check_workspace(workspace, workspace_bytes,
-                        samq_linear_grouped_workspace_v1(w, groups, x_rows, rows, x_type));
+                        samq_linear_grouped_workspace_v1(w, groups, x_rows, rows, x_type, row_index != nullptr));
         DeviceGuard guard(w->device);
         DeviceState& state = device_state(w->device);
         cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
         RoutedProduct p = routed_product(w, groups, rows, bias, epilogue, y, y_type, ldy);
-        p.row_index = row_index;
         p.offsets = offsets;
-        routed_operand(p, x, x_type, x_rows, ldx, workspace, state, stream);
+        routed_operand(p, x, x_type, x_rows, ldx, row_index, workspace, state, stream);
         launch_routed(p, state, stream);
         const_cast<samq_weights*>(w)->launches.fetch_add(1);
     });
@@ -1446,7 +1458,7 @@ samq_status samq_adapters_destroy_v1(samq_adapters* adapters) {
 
 size_t samq_linear_adapters_workspace_v1(const samq_weights* w, const samq_adapters* ad, int64_t m, int x_type) {
     if (!w || !ad || m <= 0) return 0;
-    return staged_bytes(m, w->k, x_type) + static_cast<size_t>(m) * 2 * ad->rank * sizeof(__half);
+    return operand_bytes(m, w->k, x_type == SAMQ_TYPE_F32) + static_cast<size_t>(m) * 2 * ad->rank * sizeof(__half);
 }
 
 samq_status samq_linear_adapters_v1(const samq_weights* w, const samq_adapters* ad, const void* x, int x_type,
@@ -1472,8 +1484,9 @@ samq_status samq_linear_adapters_v1(const samq_weights* w, const samq_adapters* 
         DeviceState& state = device_state(w->device);
         cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
         RoutedProduct p = routed_product(w, 1, m, bias, epilogue, y, y_type, ldy);
-        routed_operand(p, x, x_type, m, ldx, workspace, state, stream);
-        __half* h2 = reinterpret_cast<__half*>(static_cast<uint8_t*>(workspace) + staged_bytes(m, w->k, x_type));
+        routed_operand(p, x, x_type, m, ldx, nullptr, workspace, state, stream);
+        __half* h2 = reinterpret_cast<__half*>(static_cast<uint8_t*>(workspace) +
+                                             operand_bytes(m, w->k, x_type == SAMQ_TYPE_F32));
         p.ids = ids;
         p.h2 = h2;
         p.b2 = ad->b2;

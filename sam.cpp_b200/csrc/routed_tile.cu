@@ -11,11 +11,15 @@
 // gather by row index, and an index past the end reads zeros.  The pair keeps h
 // to 2^-22, f32's level against the f16 rounding of B.
 //
-// The same gather (tile::gather4, four rows an instruction, one per lane of the
-// producer warp) reads x by row_index, so no permuted copy of x is made.
+// x arrives in plan order: a row_index has been applied by gather_rows_kernel.
+// Gathering inside this kernel was measured and not kept (10368 rows of 8
+// experts, 1024 -> 4736, without GELU; 107 us in plan order, 8 us for the copy):
+// x by the row gather of TMA 287 us, by 16-byte asynchronous copies of four
+// warps 272 us (213 us when no row was to be read: the hand-over of each step to
+// the tensor core bounds it, not the memory).
 //
-// Pipeline (64 + 32 * kEpilogueWarps threads, one CTA or CTA pair per SM or TPC,
-// persistent over the tiles of all groups):
+// Pipeline (one CTA or CTA pair per SM or TPC, persistent over the tiles of all
+// groups):
 //   warp 0     producer: 128 x 64 of X and BN (a pair: BN / 2 each) x 64 of W per
 //              step by TMA, 128-byte swizzle, kStages deep.  Each step's `last`
 //              flag travels with its stage, as only the producer knows how many
@@ -55,10 +59,10 @@ struct TileSmem {
 };
 
 struct TileMaps {
-    CUtensorMap x;       // box 64 x 128 rows (x in plan order)
-    CUtensorMap x_rows;  // box 64 x 1, gathered
+    CUtensorMap x;       // box 64 x 128
     CUtensorMap w;       // box 64 x BN / CTAS
-    CUtensorMap h;       // adapters: [rows][2 rank], box 64 x 1, gathered
+    CUtensorMap h;       // adapters: [rows][2 rank], box 64 x 128
+    CUtensorMap h_rows;  // the same, box 64 x 1, gathered
     CUtensorMap b;       // adapters: [adapters * n][2 rank], box 64 x BN / CTAS
 };
 
@@ -209,46 +213,30 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         uint32_t ph = 0;
         uint32_t issued = 0, issued_phase = 0;
         bool ok = true;
-        const int nothing = static_cast<int>(p.x_rows), no_row = static_cast<int>(p.rows);  // indices that read zeros
-        // One step into the next stage: B from `bm`, A as a tile (am != null) or gathered by r from `gm`.
-        auto step = [&](const CUtensorMap* am, int arow, const CUtensorMap* gm, int4 r, const CUtensorMap* bm, int brow,
-                        int x, bool last) -> bool {
-            bool free = true;
-            if (lane == 0) free = mbar_wait(&empty[s], ph ^ 1u, status, 61);
-            if (!__shfl_sync(0xffffffffu, free, 0)) return false;
-            const uint32_t bar = CTAS == 2 ? cluster_map(&full[s], 0) : smem_u32(&full[s]);
-            if (lane == 0) {
-                if (rank == 0) {
-                    last_step[s] = last;
-                    mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
-                }
-                tma_tile<CTAS>(sb + s * L::b_bytes, bm, &full[s], bar, x, brow + rank * (BN / CTAS));
-                if (am) tma_tile<CTAS>(sa + s * L::a_bytes, am, &full[s], bar, x, arow);
+        const int no_row = static_cast<int>(p.rows);  // an index that reads zeros
+        const uint32_t full_bar = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);  // the even CTA's
+        // Lane 0: waits for the next stage, announces the step and loads B from `bm`.
+        auto open = [&](const CUtensorMap* bm, int brow, int x, bool last) -> bool {
+            if (!mbar_wait(&empty[s], ph ^ 1u, status, 61)) return false;
+            if (rank == 0) {
+                last_step[s] = last;
+                mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
             }
-            __syncwarp();
-            if (!am) tma_gather4<CTAS>(sa + s * L::a_bytes + lane * 512, gm, bar, x, r);
+            tma_tile<CTAS>(sb + s * L::b_bytes, bm, &full[s], full_bar + 8 * s, x, brow + rank * (BN / CTAS));
             issued |= 1u << s;
             issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
+            return true;
+        };
+        auto advance = [&] {
             if (++s == kStages) {
                 s = 0;
                 ph ^= 1u;
             }
-            return true;
         };
         for (int tile = unit; tile < tiles && ok; tile += units) {
             const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
             const int row0 = t.row0 + rank * BM;
             const int mine = row0 + 4 * lane;  // this lane's four rows of the CTA's 128
-            int4 src = make_int4(nothing, nothing, nothing, nothing);
-            if (p.row_index) {
-                int v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = mine + j < t.end ? __ldg(p.row_index + mine + j) : nothing;
-                    v[j] = r >= 0 && r < nothing ? r : nothing;
-                }
-                src = make_int4(v[0], v[1], v[2], v[3]);
-            }
             // The pair's 256 rows hold the same adapters for both CTAs.
             int own[4], other[4];
             int next = p.adapter_count;
@@ -263,29 +251,49 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 }
                 next = __reduce_min_sync(0xffffffffu, next);
             }
-            const int wrow = t.group * p.n + t.col0;
-            const CUtensorMap* am = p.row_index ? nullptr : &maps.x;
-            for (int kb = 0; kb < kblocks && ok; ++kb)
-                ok = step(am, row0, &maps.x_rows, src, &maps.w, wrow, kb * BK,
-                          kb == kblocks - 1 && next >= p.adapter_count);
+            if (lane == 0) {
+                const int wrow = t.group * p.n + t.col0;
+                const bool plain = next >= p.adapter_count;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    ok = open(&maps.w, wrow, kb * BK, kb == kblocks - 1 && plain);
+                    if (!ok) break;
+                    tma_tile<CTAS>(sa + s * L::a_bytes, &maps.x, &full[s], full_bar + 8 * s, kb * BK, row0);
+                    advance();
+                }
+            }
+            if (!p.ids) continue;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
             while (ok && next < p.adapter_count) {
                 const int a = next;
                 next = p.adapter_count;
                 int v[4];
+                bool all = true;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[j] = own[j] == a ? mine + j : no_row;
+                    all &= own[j] == a || mine + j >= t.end;
                     if (own[j] > a) next = min(next, own[j]);
                     if (other[j] > a) next = min(next, other[j]);
                 }
                 next = __reduce_min_sync(0xffffffffu, next);
+                all = __all_sync(0xffffffffu, all);  // no row to mask: a plain tile (rows past the end are not stored)
                 const int4 rows4 = make_int4(v[0], v[1], v[2], v[3]);
-                for (int c = 0; c < 2 * p.rank && ok; c += BK)
-                    ok = step(nullptr, 0, &maps.h, rows4, &maps.b, a * p.n + t.col0, c,
-                              c + BK >= 2 * p.rank && next >= p.adapter_count);
+                for (int c = 0; c < 2 * p.rank && ok; c += BK) {
+                    if (lane == 0) {
+                        ok = open(&maps.b, a * p.n + t.col0, c, c + BK >= 2 * p.rank && next >= p.adapter_count);
+                        if (ok && all)
+                            tma_tile<CTAS>(sa + s * L::a_bytes, &maps.h, &full[s], full_bar + 8 * s, c, row0);
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    const int stage = __shfl_sync(0xffffffffu, s, 0);
+                    if (ok && !all)
+                        tma_gather4<CTAS>(sa + stage * L::a_bytes + lane * 512, &maps.h_rows, full_bar + 8 * stage, c,
+                                          rows4);
+                    if (lane == 0 && ok) advance();
+                }
             }
         }
-        pdl_trigger();  // all loads issued
+        pdl_trigger();  // all of this warp's loads are issued
         if (!ok && lane == 0) {
             // Let the copies in flight land before the CTA exits.
             if constexpr (CTAS == 1) {
@@ -300,6 +308,8 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_f16_f32(CTAS * BM, BN);
+            // Descriptors of stage 0; a stage or 32 bytes on only moves the address field (16-byte units).
+            const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), b_desc = smem_desc_sw128(smem_u32(sb));
             int s = 0;
             uint32_t ph = 0;
             int acc = 0;
@@ -311,41 +321,35 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 if (!free) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kAccStride);
-                bool first = true, last = false;
+                uint32_t accumulate = 0;
+                bool last = false;
                 while (!last) {
-                    if (!mbar_wait(&full[s], ph, status, 63)) {
+                    const bool filled = CTAS == 2 ? mbar_wait_cluster(&full[s], ph, status, 63)
+                                                  : mbar_wait(&full[s], ph, status, 63);
+                    if (!filled) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     last = last_step[s] != 0;
-                    const uint32_t a_addr = smem_u32(sa + s * L::a_bytes);
-                    const uint32_t b_addr = smem_u32(sb + s * L::b_bytes);
+                    const uint64_t ad = a_desc + static_cast<uint32_t>(s * (L::a_bytes >> 4));
+                    const uint64_t bd = b_desc + static_cast<uint32_t>(s * (L::b_bytes >> 4));
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk) {
-                        const uint64_t ad = smem_desc_sw128(a_addr + kk * 32), bd = smem_desc_sw128(b_addr + kk * 32);
-                        if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad, bd, idesc, first ? 0u : 1u);
-                        else tc_mma_f16(d, ad, bd, idesc, first ? 0u : 1u);
-                        first = false;
+                        if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
+                        else tc_mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
+                        accumulate = 1;
                     }
-                    if constexpr (CTAS == 2) {
-                        tc_commit_pair(cluster_map(&empty[s], 0));
-                        tc_commit_pair(cluster_map(&empty[s], 1));
-                    } else {
-                        tc_commit(&empty[s]);
-                    }
+                    if constexpr (CTAS == 2) tc_commit_both(&empty[s]);
+                    else tc_commit(&empty[s]);
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
                     }
                 }
                 if (!ok) break;
-                if constexpr (CTAS == 2) {
-                    tc_commit_pair(cluster_map(&tfull[acc], 0));
-                    tc_commit_pair(cluster_map(&tfull[acc], 1));
-                } else {
-                    tc_commit(&tfull[acc]);
-                }
+                if constexpr (CTAS == 2) tc_commit_both(&tfull[acc]);
+                else tc_commit(&tfull[acc]);
                 acc ^= 1;
                 if (acc == 0) acc_ph ^= 1u;
             }
@@ -454,13 +458,13 @@ void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStre
     const auto f16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
     encode_tensor_map_2d(&maps.x, f16, p.x, p.k, p.x_rows, p.ldx * 2, BK, BM, sw);
-    encode_tensor_map_2d(&maps.x_rows, f16, p.x, p.k, p.x_rows, p.ldx * 2, BK, 1, sw);
     encode_tensor_map_2d(&maps.w, f16, p.operand, p.k, static_cast<uint64_t>(p.groups) * p.n,
                          static_cast<uint64_t>(p.k) * 2, BK, BN / CTAS, sw);
-    maps.h = maps.x_rows;
+    maps.h = maps.h_rows = maps.x;
     maps.b = maps.w;
     if (p.ids) {
-        encode_tensor_map_2d(&maps.h, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, 1, sw);
+        encode_tensor_map_2d(&maps.h, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, BM, sw);
+        encode_tensor_map_2d(&maps.h_rows, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, 1, sw);
         encode_tensor_map_2d(&maps.b, f16, p.b2, 2 * p.rank, static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank,
                              BK, BN / CTAS, sw);
     }

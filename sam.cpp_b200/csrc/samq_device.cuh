@@ -478,4 +478,13 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster_addr) {
                  : "memory");
 }
 
+// tc_commit_pair on the mbarrier at this CTA's offset of `bar` in both CTAs.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
 }  // namespace samq

@@ -445,9 +445,13 @@ struct RoutedProduct {
     const __half* b2 = nullptr;         // [adapter_count][n][2 * rank]
     int rank = 0, adapter_count = 0;
 };
+// x[row_index[i]] as the f16 operand [rows][k] (f32 x staged by the Q8_1 rule).
+void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index, int64_t rows,
+                        int k, __half* out, DeviceState& state, cudaStream_t stream);
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
                          cudaStream_t stream);
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
+constexpr int kRoutedFewRows = 64;  // rows of a group, at most, that take the packet-streaming kernel
 // routed_tile.cu: the groups of at least `min_rows` rows on tensor-core tiles.
 void launch_routed_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream);
 

@@ -185,7 +185,7 @@ SIGNATURES = {
     "samq_neck_forward_v1": (_i32, [ctypes.POINTER(NeckDesc), _vp, _i32, _i32, ctypes.POINTER(_vp), _vp]),
     "samq_route_workspace_v1": (_sz, [_i64, _i32, _i32]),
     "samq_route_v1": (_i32, [_vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "samq_linear_grouped_workspace_v1": (_sz, [_vp, _i32, _i64, _i64, _i32]),
+    "samq_linear_grouped_workspace_v1": (_sz, [_vp, _i32, _i64, _i64, _i32, _i32]),
     "samq_linear_grouped_v1": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _i64,
                                       _vp, _sz, _vp]),
     "samq_combine_v1": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _vp]),
@@ -767,8 +767,10 @@ def route(logits, tokens: int, experts: int, ld: int, top_k: int, weights, ids, 
                                        slots.data_ptr(), address, size, _stream_on(stream, device)))
 
 
-def linear_grouped_workspace(w: Weights, groups: int, x_rows: int, rows: int, x_dtype) -> int:
-    return library().samq_linear_grouped_workspace_v1(w.handle, groups, x_rows, rows, _element(x_dtype))
+def linear_grouped_workspace(w: Weights, groups: int, x_rows: int, rows: int, x_dtype, indexed: bool = True) -> int:
+    """Bytes of workspace a call needs; `indexed`: with a row_index (never less than without)."""
+    return library().samq_linear_grouped_workspace_v1(w.handle, groups, x_rows, rows, _element(x_dtype),
+                                                      1 if indexed else 0)
 
 
 def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, rows: int, y, ldy: int, row_index=None,
@@ -778,7 +780,8 @@ def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, r
     device = _same_device(w.device, x, offsets, y, row_index, bias)
     _int32(offsets, row_index)
     xt, yt = _element(x.dtype), _element(y.dtype)
-    needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt)
+    needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt,
+                                                                            row_index is not None)
     keep, address, size = _scratch(workspace, needed, device)
     _check(library().samq_linear_grouped_v1(w.handle, groups, x.data_ptr(), xt, x_rows, ldx, _addr(row_index),
                                             offsets.data_ptr(), rows, _addr(bias), epilogue, y.data_ptr(), yt, ldy,

@@ -68,7 +68,7 @@ def test_linears_refuse_null_handles(samq):
             "null weights")
     refused(samq, "samq_adapters_set_v1", [None, 0, 0, None, None, 1, 1.0, None], "null adapters")
     lib = samq.library()
-    assert lib.samq_linear_grouped_workspace_v1(None, 1, 8, 8, 0) == 0
+    assert lib.samq_linear_grouped_workspace_v1(None, 1, 8, 8, 0, 1) == 0
     assert lib.samq_linear_adapters_workspace_v1(None, None, 8, 0) == 0
     assert lib.samq_adapters_destroy_v1(None) == 0
 
