@@ -25,9 +25,10 @@
 //              flag travels with its stage, as only the producer knows how many
 //              adapters a tile has;
 //   warp 1     TMEM owner; one thread (of the even CTA) issues tcgen05.mma;
-//   warps 2..  epilogue: accumulator out of TMEM, bias, erf-GELU, stores of 32
-//              bytes a lane (a whole L2 sector) straight from registers, rows
-//              past the group's end left alone.  The next tile's MMAs overlap it.
+//   warps 2..  epilogue: accumulator out of TMEM, bias, erf-GELU, 32 rows of 128
+//              bytes at a time through swizzled shared memory: one TMA store, or,
+//              where the group ends inside them, coalesced stores of its own rows.
+//              The next tile's MMAs overlap it.
 // Every wait is bounded.  No load uses multicast.
 #include <algorithm>
 
@@ -39,22 +40,26 @@ namespace {
 constexpr int BM = 128;  // rows of a CTA's tile
 constexpr int BK = 64;   // depth of a step: one 128-byte swizzle row of f16
 constexpr int kAccStride = 256;
-constexpr int kEpilogueWarps = 16;
+constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kMaxGroups = 1024;
+constexpr int kSlabBytes = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int kSmemLimit = 232448;
 
-template <int CTAS, int BN>
+// GROUPS: the most groups the tables hold.  They take a stage's room only in
+// the instance for many groups.
+template <int CTAS, int BN, int GROUPS>
 struct TileSmem {
     static constexpr int a_bytes = BM * BK * 2;
     static constexpr int b_bytes = BN / CTAS * BK * 2;
     static constexpr int stage = a_bytes + b_bytes;
-    static constexpr int tables = 3 * (kMaxGroups + 1) * 4;  // tile prefix, begin, end of each group
-    static constexpr int fixed = 1024 + tables + 512;
+    static constexpr int out = kEpilogueWarps * kSlabBytes;
+    static constexpr int tables = (3 * GROUPS + 1) * 4;  // begin, end, tile prefix of each group
+    static constexpr int fixed = 1024 + out + tables + 256;
     static constexpr int stages = (kSmemLimit - fixed) / stage > 8 ? 8 : (kSmemLimit - fixed) / stage;
     static constexpr int b_off = stages * a_bytes;
-    static constexpr int table_off = stages * stage;
-    static constexpr int bar_off = (table_off + tables + 15) / 16 * 16;
+    static constexpr int out_off = stages * stage;
+    static constexpr int bar_off = out_off + out;
+    static constexpr int table_off = bar_off + 256;
     static constexpr int total = stages * stage + fixed;
 };
 
@@ -64,6 +69,7 @@ struct TileMaps {
     CUtensorMap h;       // adapters: [rows][2 rank], box 64 x 128
     CUtensorMap h_rows;  // the same, box 64 x 1, gathered
     CUtensorMap b;       // adapters: [adapters * n][2 rank], box 64 x BN / CTAS
+    CUtensorMap y;       // output, box 128 bytes x 32
 };
 
 // Four rows of 64 columns by index into shared memory (the map's box is one row
@@ -89,18 +95,6 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
                                          int y) {
     if constexpr (CTAS == 1) tma_load_2d(dst, map, local, x, y);
     else tma_load_2d_pair(dst, map, bar, x, y);
-}
-
-// 32 bytes of one row: a whole L2 sector where the row allows it.
-__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8], bool wide) {
-    if (wide) {
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
-                     "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                     : "memory");
-    } else {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
-        *(reinterpret_cast<uint4*>(dst) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
-    }
 }
 
 __device__ __forceinline__ int clamp_row(int v, int64_t rows) {
@@ -129,20 +123,20 @@ __device__ __forceinline__ Tile find_tile(int tile, int n_tiles, int bn, int row
     return t;
 }
 
-template <int CTAS, int BN>
+template <int CTAS, int BN, int GROUPS>
 __global__ void __launch_bounds__(kThreads, 1)
 routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p, int min_rows, DeviceStatus* status) {
-    using L = TileSmem<CTAS, BN>;
+    using L = TileSmem<CTAS, BN, GROUPS>;
     constexpr int kStages = L::stages;
     static_assert(kStages >= 3 && L::total <= kSmemLimit, "shared memory budget");
-    static_assert(2 * 8 * kStages + 5 * 8 + 8 + 4 * kStages <= 512, "barrier space");
+    static_assert(2 * 8 * kStages + 5 * 8 + 8 + 4 * kStages <= 256, "barrier space");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sa = smem;
     uint8_t* sb = smem + L::b_off;
-    int* s_first = reinterpret_cast<int*>(smem + L::table_off);
-    int* s_begin = s_first + kMaxGroups + 1;
-    int* s_end = s_begin + kMaxGroups + 1;
+    int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
+    int* s_end = s_begin + GROUPS;
+    int* s_first = s_end + GROUPS;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
     uint64_t* empty = full + kStages;
     uint64_t* tfull = empty + kStages;
@@ -171,6 +165,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         fence_barrier_init();
         tma_prefetch_desc(&maps.x);
         tma_prefetch_desc(&maps.w);
+        tma_prefetch_desc(&maps.y);
     }
     if (warp == 1) {
         if constexpr (CTAS == 2) tmem_alloc_pair(tmem_slot, 2 * kAccStride);
@@ -360,74 +355,106 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         }
         __syncwarp();
     } else {
-        constexpr int kParts = kEpilogueWarps / 4;
-        constexpr int kChunks = BN / 32;
-        const int quarter = warp & 3;      // TMEM lanes 32 * quarter ..
-        const int part = (warp - 2) >> 2;  // its share of the columns
+        constexpr int kShare = BN / (kEpilogueWarps / 4);  // columns of a warp
+        const int quarter = warp & 3;                      // TMEM lanes 32 * quarter ..
+        const int part = (warp - 2) >> 2;
         const bool f16 = p.y_type == SAMQ_TYPE_F16;
         const int elem = f16 ? 2 : 4;
-        const bool vec = p.ldy * elem % 16 == 0;
-        const bool wide = p.ldy * elem % 32 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31u) == 0;
+        const int slab_cols = 128 / elem;
+        uint8_t* slab = smem + L::out_off + (warp - 2) * kSlabBytes;
         int acc = 0;
         uint32_t acc_ph = 0;
         for (int tile = unit; tile < tiles; tile += units) {
             const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
-            const int row = t.row0 + rank * BM + quarter * 32 + lane;
+            const int row0 = t.row0 + rank * BM + quarter * 32;
+            const float* bias = p.bias ? p.bias + static_cast<int64_t>(t.group) * p.n + t.col0 : nullptr;
+            const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15u) == 0;
             // Warp-uniform: the TMEM loads below are warp-collective.
             if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 64))) break;
             tc_fence_after();
-            uint8_t* out = static_cast<uint8_t*>(p.y) + (static_cast<int64_t>(row) * p.ldy + t.col0) * elem;
-            const float* bias = p.bias ? p.bias + static_cast<int64_t>(t.group) * p.n + t.col0 : nullptr;
 #pragma unroll 1
-            for (int c = part * kChunks / kParts * 32; c < (part + 1) * kChunks / kParts * 32; c += 32) {
-                const int left = p.n - t.col0 - c;  // columns of this chunk inside the group
-                if (left <= 0) break;
-                const float bias_lane = bias && lane < left ? __ldg(bias + c + lane) : 0.0f;
-                uint32_t r[32];
-                tc_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                     static_cast<uint32_t>(acc * kAccStride + c),
-                                 r);
-                tc_wait_ld();
-                float v[32];
+            for (int c0 = part * kShare; c0 < (part + 1) * kShare; c0 += slab_cols) {
+                const int inside = p.n - t.col0 - c0;  // columns from here to the group's last
+                if (inside <= 0 || row0 >= t.end) break;
+                if (lane == 0) bulk_wait_group_read<0>();  // the slab's last store has left it
+                __syncwarp();
+#pragma unroll 1
+                for (int c = c0; c < c0 + slab_cols; c += 32) {
+                    const int left = p.n - t.col0 - c;
+                    uint32_t r[32];
+                    tc_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                         static_cast<uint32_t>(acc * kAccStride + c),
+                                     r);
+                    float v[32];
+                    if (bias && left >= 32 && bias_vec) {
+                        const float4* b4 = reinterpret_cast<const float4*>(bias + c);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + __shfl_sync(0xffffffffu, bias_lane, i);
-                if (p.gelu) {
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 b = __ldg(b4 + j);
+                            v[4 * j] = b.x; v[4 * j + 1] = b.y; v[4 * j + 2] = b.z; v[4 * j + 3] = b.w;
+                        }
+                    } else {
+                        const float mine = bias && lane < left ? __ldg(bias + c + lane) : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = gelu_erf(v[i]);
-                }
-                if (row < t.end) {
-                    if (left >= 32 && vec) {
-                        if (f16) {
+                        for (int i = 0; i < 32; ++i) v[i] = __shfl_sync(0xffffffffu, mine, i);
+                    }
+                    tc_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                uint32_t o[8];
+                    for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(r[i]);
+                    if (p.gelu) {
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const __half2 h = __floats2half2_rn(v[16 * j + 2 * i], v[16 * j + 2 * i + 1]);
-                                    o[i] = *reinterpret_cast<const uint32_t*>(&h);
-                                }
-                                store32(out + c * 2 + 32 * j, o, wide);
+                        for (int i = 0; i < 32; ++i) v[i] = gelu_erf(v[i]);
+                    }
+                    // 16-byte unit u of row `lane` at u ^ (lane % 8): the store's 128-byte swizzle.
+                    if (f16) {
+                        const int u0 = (c - c0) >> 3;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const __half2 h = __floats2half2_rn(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+                                o[i] = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t o[8];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[8 * j + i]);
-                                store32(out + c * 4 + 32 * j, o, wide);
-                            }
+                            *reinterpret_cast<uint4*>(slab + lane * 128 + (((u0 + j) ^ (lane & 7)) << 4)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (i < left) {
-                                if (f16) reinterpret_cast<__half*>(out)[c + i] = __float2half_rn(v[i]);
-                                else reinterpret_cast<float*>(out)[c + i] = v[i];
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4*>(slab + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                }
+                if (row0 + 32 <= t.end) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&maps.y, slab, t.col0 + c0, row0);  // clipped at column n
+                        bulk_commit_group();
+                    }
+                } else {
+                    // Another group's rows (or the caller's) follow: 8 lanes a row, the group's own rows only.
+                    __syncwarp();
+                    const int u = lane & 7, units_inside = min(inside, slab_cols) * elem / 16;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = 4 * i + (lane >> 3);
+                        if (row0 + rr >= t.end) continue;
+                        const uint8_t* from = slab + rr * 128 + ((u ^ (rr & 7)) << 4);
+                        uint8_t* to = static_cast<uint8_t*>(p.y) +
+                                      (static_cast<int64_t>(row0 + rr) * p.ldy + t.col0 + c0) * elem + 16 * u;
+                        if (u < units_inside) {
+                            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                        } else if (u == units_inside) {
+                            for (int b = 0; b < (inside * elem) % 16 && inside < slab_cols; b += elem) {
+                                if (f16) *reinterpret_cast<__half*>(to + b) = *reinterpret_cast<const __half*>(from + b);
+                                else *reinterpret_cast<float*>(to + b) = *reinterpret_cast<const float*>(from + b);
                             }
                         }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();  // converged for the next chunk's collective TMEM load
             }
             tc_fence_before();
             __syncwarp();
@@ -438,6 +465,9 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             acc ^= 1;
             if (acc == 0) acc_ph ^= 1u;
         }
+        // The CTA may exit once its stores have read their shared memory.
+        if (lane == 0) bulk_wait_group_read<0>();
+        __syncwarp();
     }
     tc_fence_before();
     __syncwarp();
@@ -451,15 +481,19 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
     }
 }
 
-template <int CTAS, int BN>
+template <int CTAS, int BN, int GROUPS>
 void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
-    using L = TileSmem<CTAS, BN>;
+    using L = TileSmem<CTAS, BN, GROUPS>;
     TileMaps maps;
     const auto f16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
     encode_tensor_map_2d(&maps.x, f16, p.x, p.k, p.x_rows, p.ldx * 2, BK, BM, sw);
     encode_tensor_map_2d(&maps.w, f16, p.operand, p.k, static_cast<uint64_t>(p.groups) * p.n,
                          static_cast<uint64_t>(p.k) * 2, BK, BN / CTAS, sw);
+    if (p.y_type == SAMQ_TYPE_F16)
+        encode_tensor_map_2d(&maps.y, f16, p.y, p.n, p.rows, p.ldy * 2, 64, 32, sw);
+    else
+        encode_tensor_map_2d(&maps.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, p.y, p.n, p.rows, p.ldy * 4, 32, 32, sw);
     maps.h = maps.h_rows = maps.x;
     maps.b = maps.w;
     if (p.ids) {
@@ -468,7 +502,7 @@ void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStre
         encode_tensor_map_2d(&maps.b, f16, p.b2, 2 * p.rank, static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank,
                              BK, BN / CTAS, sw);
     }
-    auto kernel = routed_tile_kernel<CTAS, BN>;
+    auto kernel = routed_tile_kernel<CTAS, BN, GROUPS>;
     const void* fn = reinterpret_cast<const void*>(kernel);
     set_smem_limit_once(state, fn, L::total, "cudaFuncSetAttribute(routed tile smem)");
     const int64_t tiles = (p.rows / (CTAS * BM) + p.groups) * ((p.n + BN - 1) / BN);  // at most
@@ -485,11 +519,17 @@ void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStre
     }
 }
 
+template <int GROUPS>
+void run_shape(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
+    if (p.rows >= 256 * p.groups) run_tile<2, 256, GROUPS>(p, min_rows, state, stream);
+    else run_tile<1, 128, GROUPS>(p, min_rows, state, stream);
+}
+
 }  // namespace
 
 void launch_routed_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
-    if (p.rows >= 256 * p.groups) run_tile<2, 256>(p, min_rows, state, stream);
-    else run_tile<1, 128>(p, min_rows, state, stream);
+    if (p.groups <= 128) run_shape<128>(p, min_rows, state, stream);
+    else run_shape<1024>(p, min_rows, state, stream);
 }
 
 }  // namespace samq
