@@ -1,88 +1,15 @@
 // grouped.cu -- products whose weight depends on the row (samq_linear_grouped_v1,
 // samq_linear_adapters_v1): y[i] = act(W_g x[row_index[i]] + bias_g + delta_i)
-// for the rows i of group g, with delta the row's low-rank adapter.
+// for the rows i of group g, with delta the row's low-rank adapter.  Here the
+// operand in plan order, the adapters' down product and the choice of kernel;
+// the products themselves are in routed_rows.cu and routed_tile.cu.
 #include <algorithm>
+#include <climits>
 
 #include "samq_internal.hpp"
 
 namespace samq {
 namespace {
-
-constexpr int kTile = 64;      // rows and columns of a block's tile
-constexpr int kDepth = 16;     // depth of a step
-constexpr int kThreads = 256;  // 16 x 16 threads, 4 x 4 outputs each
-
-__device__ __forceinline__ int clamp_offset(const int* offsets, int g, int64_t rows) {
-    const int64_t v = offsets[g];
-    return static_cast<int>(v < 0 ? 0 : v > rows ? rows : v);
-}
-
-// Tile (blockIdx.x: columns, blockIdx.y: the n-th row tile over all groups).
-template <class OUT>
-__global__ void __launch_bounds__(kThreads) grouped_kernel(const RoutedProduct p) {
-    __shared__ float sx[kDepth][kTile + 1], sw[kDepth][kTile + 1];
-    __shared__ int s_row0, s_end, s_group;
-    pdl_wait();
-    pdl_trigger();
-    if (threadIdx.x == 0) {
-        int left = blockIdx.y, g = 0, begin = 0, end = 0;
-        for (; g < p.groups; ++g) {
-            begin = p.offsets ? clamp_offset(p.offsets, g, p.rows) : 0;
-            end = p.offsets ? max(begin, clamp_offset(p.offsets, g + 1, p.rows)) : static_cast<int>(p.rows);
-            const int tiles = (end - begin + kTile - 1) / kTile;
-            if (left < tiles) break;
-            left -= tiles;
-        }
-        s_group = g;
-        s_row0 = begin + left * kTile;
-        s_end = end;
-    }
-    __syncthreads();
-    const int group = s_group, row0 = s_row0, end = s_end;
-    if (group >= p.groups) return;
-    const int col0 = blockIdx.x * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const __half* w = p.operand + static_cast<int64_t>(group) * p.n * p.k;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.k; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kThreads) {
-            const int r = i / kDepth, c = i % kDepth;
-            int64_t src = row0 + r < end ? row0 + r : -1;
-            if (src >= 0 && p.row_index) src = p.row_index[src];
-            const bool in = k0 + c < p.k;
-            sx[c][r] = in && src >= 0 && src < p.x_rows ? __half2float(p.x[src * p.ldx + k0 + c]) : 0.0f;
-            sw[c][r] = in && col0 + r < p.n ? __half2float(w[static_cast<int64_t>(col0 + r) * p.k + k0 + c]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kDepth; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sx[c][ty + 16 * i], sw[c][tx + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i) {
-        const int row = row0 + ty + 16 * i;
-        if (row >= end) continue;
-        const int a = p.ids ? p.ids[row] : -1;
-        const bool adapted = p.ids && a >= 0 && a < p.adapter_count;
-        for (int j = 0; j < 4; ++j) {
-            const int col = col0 + tx + 16 * j;
-            if (col >= p.n) continue;
-            float v = acc[i][j] + (p.bias ? p.bias[static_cast<int64_t>(group) * p.n + col] : 0.0f);
-            if (adapted) {
-                const __half* b = p.b2 + (static_cast<int64_t>(a) * p.n + col) * 2 * p.rank;
-                const __half* h = p.h2 + static_cast<int64_t>(row) * 2 * p.rank;
-                float d = 0.0f;
-                for (int r = 0; r < 2 * p.rank; ++r) d = fmaf(__half2float(h[r]), __half2float(b[r]), d);
-                v += d;
-            }
-            if (p.gelu) v = gelu_erf(v);
-            static_cast<OUT*>(p.y)[static_cast<int64_t>(row) * p.ldy + col] = static_cast<OUT>(v);
-        }
-    }
-}
 
 // h2[i] = hi | lo of scale_a A_a x[i]: one warp per (row, rank index).
 __global__ void __launch_bounds__(256) adapter_down_kernel(const RoutedProduct p, const __half* __restrict__ a_all,
@@ -175,17 +102,14 @@ void launch_adapter_down(const RoutedProduct& p, const samq_adapters& ad, __half
                static_cast<const int*>(ad.ranks), h2, state.status);
 }
 
+// Few rows stream the packets, many take the f16 tiles.  Between, a call holds
+// groups of either kind and only the device knows which: both kernels run and
+// each leaves the other's groups alone.
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream) {
-    if (p.rows > 64) {
-        launch_routed_tile(p, 1, state, stream);
-        return;
-    }
-    const int64_t tiles = std::min<int64_t>(p.rows, p.rows / kTile + p.groups);
-    const dim3 grid(static_cast<unsigned>((p.n + kTile - 1) / kTile), static_cast<unsigned>(tiles));
-    if (p.y_type == SAMQ_TYPE_F16)
-        launch_pdl(grouped_kernel<__half>, grid, dim3(kThreads), 0, stream, "grouped_kernel launch", p);
-    else
-        launch_pdl(grouped_kernel<float>, grid, dim3(kThreads), 0, stream, "grouped_kernel launch", p);
+    const bool few = p.rows <= kRoutedFewRows;
+    const bool many = !few && (p.groups == 1 || p.rows >= 256 * p.groups);
+    if (!many) launch_routed_rows(p, few ? INT_MAX : kRoutedFewRows, state, stream);
+    if (!few) launch_routed_tile(p, many ? 1 : kRoutedFewRows + 1, state, stream);
 }
 
 }  // namespace samq

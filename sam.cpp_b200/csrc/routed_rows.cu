@@ -1,0 +1,625 @@
+// routed_rows.cu -- the routed product for groups of few rows (decoding): the
+// packed weights of the groups in use stream through once and are decoded on the
+// way, so HBM carries 0.56-1.06 bytes a weight instead of the 2 of the f16
+// expansion the tiles of routed_tile.cu read.
+//
+// y[i] = act(W_g x[i] + bias_g + delta_i) with the factors swapped: a unit is one
+// packet row tile (128 rows of the stacked weights) of one group by up to TOK of
+// the group's rows, D[128][TOK] = W_tile . X^T in TMEM (tcgen05.mma M = 128,
+// N = TOK).  What bounds it at full size is the packet stream; what bounds it at
+// a few rows is the chain of one unit, so a cluster of SPLIT CTAs shares a unit's
+// depth and adds its partial sums over distributed shared memory, in rank order:
+// one launch, no atomics, no workspace.
+//
+// One CTA per SM, persistent over the units of all groups:
+//   warp 0       each step's packet by a bulk copy, its 64 columns of X by TMA (rows
+//                by index through the row gather), kStages deep;
+//   warp 1       TMEM owner; one thread issues the MMAs;
+//   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
+//                shared memory and back, summed over the cluster), bias, adapters,
+//                erf-GELU, stores coalesced over the weight rows;
+//   warps 6-21   decoders, two sets of eight on alternate steps: a thread turns 32
+//                columns of a row into f16 with the values of packets.cuh bit for bit.
+// The decoders are the busiest pipe, hence their arithmetic: a nibble becomes a
+// float by or-ing it into the mantissa of 2^23 where it stands (the sub-block's
+// scale takes the power of 16), and pairs of weights share packed f32 operations;
+// an int8 becomes a half by the same trick with 1024, and f16(q d) needs a
+// single half multiplication as q d has at most 19 bits.
+// Every wait is bounded.  No load uses multicast.
+#include <algorithm>
+#include <climits>
+#include <map>
+#include <tuple>
+
+#include "packets.cuh"
+#include "samq_internal.hpp"
+
+namespace samq {
+namespace {
+
+constexpr int kDecodeWarps = 16;
+constexpr int kThreads = 32 * (6 + kDecodeWarps);
+constexpr int kABuffers = 4;
+constexpr int kMaxGroups = 1024;
+constexpr int kSmemLimit = 232448;
+constexpr int kMaxSplit = 8;
+
+template <int TYPE, int TOK>
+struct RowsSmem {
+    static constexpr int raw_bytes = 128 * (code_bytes_of(TYPE) + 8);  // one packet
+    static constexpr int x_bytes = TOK * 128;
+    static constexpr int a_bytes = 128 * 128;
+    static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
+    static constexpr int tables = (3 * kMaxGroups + 1) * 4;
+    static constexpr int fixed = 1024 + kABuffers * a_bytes + part + 512 + tables;
+    static constexpr int stages = (kSmemLimit - fixed) / (raw_bytes + x_bytes) > 12
+                                      ? 12
+                                      : (kSmemLimit - fixed) / (raw_bytes + x_bytes);
+    static constexpr int x_off = kABuffers * a_bytes;
+    static constexpr int raw_off = x_off + stages * x_bytes;
+    static constexpr int part_off = raw_off + stages * raw_bytes;
+    static constexpr int bar_off = part_off + part;
+    static constexpr int table_off = bar_off + 512;
+    static constexpr int total = fixed + stages * (raw_bytes + x_bytes);
+};
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_of(uint64_t v) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float half_at(const uint8_t* p) {
+    return __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(p)));
+}
+
+// Columns 32 h .. 32 h + 31 of a packet row as f16: word i of `out` holds columns
+// 2 i and 2 i + 1 of the 32.
+template <int TYPE>
+__device__ __forceinline__ void decode32(const uint8_t* __restrict__ code, const uint8_t* __restrict__ rec, int h,
+                                         uint32_t (&out)[16]) {
+    if constexpr (TYPE == SAMQ_TYPE_Q8_0) {
+        const __half2 d = __half2half2(__ushort_as_half(*reinterpret_cast<const uint16_t*>(rec + 2 * h)));
+        const __half2 bias = __floats2half2_rn(-1152.0f, -1152.0f);  // 1024 of the mantissa trick, 128 of the sign
+        uint32_t w[8];
+        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(code + 32 * h);
+        *reinterpret_cast<uint4*>(w + 4) = *reinterpret_cast<const uint4*>(code + 32 * h + 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t u = w[i] ^ 0x80808080u;
+            const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+            const __half2 a = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&lo), bias), d);
+            const __half2 b = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&hi), bias), d);
+            out[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+            out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    } else {
+        // Words of 8 nibbles (column 8 j + i at bit 4 i).
+        uint32_t lo[4];
+        if constexpr (TYPE == SAMQ_TYPE_Q5_K) {  // 40-byte rows
+            *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(code + 16 * h);
+            *reinterpret_cast<uint2*>(lo + 2) = *reinterpret_cast<const uint2*>(code + 16 * h + 8);
+        } else {
+            *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(code + 16 * h);
+        }
+        // Column i of a word's lower (upper, shifted down) half stands at bit 4 (i % 4): worth 16^(i % 4) in the
+        // mantissa of 2^23, where up to 23 bits are free.
+        constexpr uint32_t kMagic = 0x4b000000u;
+        const float d = half_at(rec);
+        if constexpr (TYPE == SAMQ_TYPE_Q6_K) {
+            const uint2 hi = *reinterpret_cast<const uint2*>(code + 32 + 8 * h);  // 2 bits a column
+            const uint64_t off01 = pack2(-8388608.0f - 32.0f, -8388608.0f - 512.0f);
+            const uint64_t off23 = pack2(-8388608.0f - 8192.0f, -8388608.0f - 131072.0f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float ds = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(rec[2 + 2 * h + (j >> 1)])));
+                const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
+                const uint32_t bits = ((j & 2) ? hi.y : hi.x) >> (16 * (j & 1));
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t n = lo[j] >> (16 * q), b = (bits >> (8 * q)) & 0xffu;
+                    // the two high bits of column i, at bit 4 i + 4
+                    const uint32_t v0 = (n & 0xfu) | ((b << 4) & 0x30u) | kMagic;
+                    const uint32_t v1 = (n & 0xf0u) | ((b << 6) & 0x300u) | kMagic;
+                    const uint32_t v2 = (n & 0xf00u) | ((b << 8) & 0x3000u) | kMagic;
+                    const uint32_t v3 = (n & 0xf000u) | ((b << 10) & 0x30000u) | kMagic;
+                    out[4 * j + 2 * q] = half2_of(mul2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off01), s01));
+                    out[4 * j + 2 * q + 1] =
+                        half2_of(mul2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off23), s23));
+                }
+            }
+        } else {
+            const float ds = __fmul_rn(d, static_cast<float>(rec[4 + h]));
+            const float dm = __fmul_rn(half_at(rec + 2), static_cast<float>(rec[6 + h]));
+            const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
+            const uint64_t m2 = pack2(-dm, -dm), off = pack2(-8388608.0f, -8388608.0f);
+            uint32_t high = 0;
+            if constexpr (TYPE == SAMQ_TYPE_Q5_K) high = *reinterpret_cast<const uint32_t*>(code + 32 + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t n = lo[j] >> (16 * q);
+                    uint32_t v0 = (n & 0xfu) | kMagic, v1 = (n & 0xf0u) | kMagic;
+                    uint32_t v2 = (n & 0xf00u) | kMagic, v3 = (n & 0xf000u) | kMagic;
+                    if constexpr (TYPE == SAMQ_TYPE_Q5_K) {
+                        const uint32_t b = high >> (8 * j + 4 * q);
+                        v0 |= (b << 4) & 0x10u;
+                        v1 |= (b << 7) & 0x100u;
+                        v2 |= (b << 10) & 0x1000u;
+                        v3 |= (b << 13) & 0x10000u;
+                    }
+                    // ds q has at most 22 bits, so the fused form rounds where the separate one does
+                    out[4 * j + 2 * q] =
+                        half2_of(fma2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off), s01, m2));
+                    out[4 * j + 2 * q + 1] =
+                        half2_of(fma2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off), s23, m2));
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int x, const int (&r)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+        "%5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int clamp_row(int v, int64_t rows) {
+    return v < 0 ? 0 : v > rows ? static_cast<int>(rows) : v;
+}
+
+// Packet row tiles that hold rows of group g.
+__device__ __forceinline__ int first_tile(int g, int n) { return static_cast<int>(static_cast<int64_t>(g) * n / 128); }
+__device__ __forceinline__ int group_tiles(int g, int n) {
+    return static_cast<int>((static_cast<int64_t>(g + 1) * n - 1) / 128) - first_tile(g, n) + 1;
+}
+
+struct Unit {
+    int group, tile, row0, count;  // packet row tile of the stacked weights, plan rows row0 .. row0 + count - 1
+};
+
+template <int TOK>
+__device__ __forceinline__ Unit find_unit(int unit, int n, int groups, const int* s_first, const int* s_begin,
+                                          const int* s_end) {
+    int lo = 0, hi = groups;  // s_first[lo] <= unit < s_first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    const int tiles = group_tiles(lo, n), at = unit - s_first[lo];
+    Unit u;
+    u.group = lo;
+    u.tile = first_tile(lo, n) + at % tiles;
+    u.row0 = s_begin[lo] + at / tiles * TOK;
+    u.count = min(TOK, s_end[lo] - u.row0);
+    return u;
+}
+
+template <int TYPE, int TOK>
+__global__ void __launch_bounds__(kThreads, 1)
+routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduct p, int max_rows, int split,
+                   DeviceStatus* status) {
+    using L = RowsSmem<TYPE, TOK>;
+    constexpr int kStages = L::stages;
+    static_assert(kStages >= 4 && L::total <= kSmemLimit, "shared memory budget");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sa = smem;
+    uint8_t* sx = smem + L::x_off;
+    uint8_t* sraw = smem + L::raw_off;
+    float* spart = reinterpret_cast<float*>(smem + L::part_off);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
+    uint64_t* empty = full + kStages;
+    uint64_t* a_full = empty + kStages;
+    uint64_t* a_empty = a_full + kABuffers;
+    uint64_t* tfull = a_empty + kABuffers;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* part_full = tempty + 2;   // every CTA of the cluster has written its partial sums
+    uint64_t* part_free = part_full + 1;  // every CTA has read this one's
+    uint64_t* drain = part_free + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    static_assert((2 * kStages + 2 * kABuffers + 4 + 3) * 8 + 4 <= 512, "barrier space");
+    int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
+    int* s_end = s_begin + kMaxGroups;
+    int* s_first = s_end + kMaxGroups;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+    const int cluster = blockIdx.x / split, clusters = gridDim.x / split;
+    const int chunks = (p.k + 63) / 64;
+    const int per = (chunks + split - 1) / split;  // steps of a rank (the host leaves none without)
+    const int c_begin = rank * per, steps = min(chunks, c_begin + per) - c_begin;
+    constexpr uint32_t kTmemCols = 2 * TOK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < kABuffers; ++b) {
+            mbar_init(&a_full[b], kDecodeWarps / 2);
+            mbar_init(&a_empty[b], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 4);
+        }
+        mbar_init(part_full, 4 * split);
+        mbar_init(part_free, 4 * split);
+        mbar_init(drain, 1);
+        fence_barrier_init();
+        tma_prefetch_desc(&map_x);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
+    // What the previous kernel may write is read from here on.
+    pdl_wait();
+    if (warp == 2) {
+        int carry = 0;
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + lane;
+            int begin = 0, end = 0, units = 0;
+            if (g < p.groups) {
+                begin = p.offsets ? clamp_row(__ldg(p.offsets + g), p.rows) : 0;
+                end = p.offsets ? max(begin, clamp_row(__ldg(p.offsets + g + 1), p.rows)) : static_cast<int>(p.rows);
+                units = end - begin <= max_rows ? (end - begin + TOK - 1) / TOK * group_tiles(g, p.n) : 0;
+                s_begin[g] = begin;
+                s_end[g] = end;
+            }
+            int sum = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            if (g < p.groups) s_first[g] = carry + sum - units;
+            carry += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) s_first[p.groups] = carry;
+    }
+    tc_fence_before();
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int units = s_first[p.groups];
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        uint32_t issued = 0, issued_phase = 0;
+        bool ok = true;
+        for (int unit = cluster; unit < units && ok; unit += clusters) {
+            const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
+            const uint8_t* packet = p.packets + (static_cast<int64_t>(u.tile) * chunks + c_begin) * L::raw_bytes;
+            int rows[4];
+            if (p.row_index && lane < TOK / 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * lane + j < u.count ? __ldg(p.row_index + u.row0 + 4 * lane + j) : -1;
+                    rows[j] = r >= 0 && r < p.x_rows ? r : static_cast<int>(p.x_rows);  // past the end: zeros
+                }
+            }
+            for (int i = 0; i < steps && ok; ++i) {
+                if (lane == 0) {
+                    ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
+                    if (ok) {
+                        mbar_arrive_expect_tx(&full[s], L::raw_bytes + L::x_bytes);
+                        bulk_load_1d(sraw + s * L::raw_bytes, packet + static_cast<int64_t>(i) * L::raw_bytes,
+                                     L::raw_bytes, &full[s]);
+                        if (!p.row_index)
+                            tma_load_2d(sx + s * L::x_bytes, &map_x, &full[s], (c_begin + i) * 64, u.row0);
+                    }
+                }
+                if (p.row_index) {
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (ok && lane < TOK / 4)
+                        gather4(sx + s * L::x_bytes + lane * 512, &map_x, &full[s], (c_begin + i) * 64, rows);
+                }
+                if (!ok) break;
+                issued |= 1u << s;
+                issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
+                if (++s == kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        pdl_trigger();  // all loads issued
+        if (!ok && lane == 0) {  // let the copies in flight land before the CTA exits
+            for (int i = 0; i < kStages; ++i)
+                if (issued & (1u << i)) mbar_wait(&full[i], (issued_phase >> i) & 1u, status, 75);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_f16_f32(128, TOK);
+            const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), x_desc = smem_desc_sw128(smem_u32(sx));
+            int s = 0, ab = 0, acc = 0;
+            uint32_t ph = 0, ab_ph = 0, acc_ph = 0;
+            bool ok = true;
+            for (int unit = cluster; unit < units && ok; unit += clusters) {
+                if (!mbar_wait(&tempty[acc], acc_ph ^ 1u, status, 72)) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TOK);
+                for (int i = 0; i < steps; ++i) {
+                    if (!mbar_wait(&full[s], ph, status, 73) || !mbar_wait(&a_full[ab], ab_ph, status, 74)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t ad = a_desc + static_cast<uint32_t>(ab * (L::a_bytes >> 4));
+                    const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc_mma_f16(d, ad + 2 * kk, xd + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
+                    tc_commit(&empty[s]);
+                    tc_commit(&a_empty[ab]);
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                    if (++ab == kABuffers) {
+                        ab = 0;
+                        ab_ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                tc_commit(&tfull[acc]);
+                acc ^= 1;
+                if (acc == 0) acc_ph ^= 1u;
+            }
+            tc_commit(drain);  // every MMA this thread issued is complete before TMEM is released
+            mbar_wait(drain, 0, status, 76);
+        }
+        __syncwarp();
+    } else if (warp >= 6) {
+        // Step q of the CTA (over all its units) goes to set q & 1, buffer q % kABuffers.
+        const int set = (warp - 6) >> 3;
+        const int id = ((warp - 6) & 7) * 32 + lane;
+        const int r = id >> 1, h = id & 1;
+        int s = set, ab = set;  // stage and buffer of this set's next step (kStages >= 2)
+        uint32_t ph = 0, ab_ph = 0;
+        const int my_units = units > cluster ? (units - cluster + clusters - 1) / clusters : 0;
+        const int total = my_units * steps;
+        for (int q = set; q < total; q += 2) {
+            const bool ok = mbar_wait(&full[s], ph, status, 77) && mbar_wait(&a_empty[ab], ab_ph ^ 1u, status, 78);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const uint8_t* raw = sraw + s * L::raw_bytes;
+            uint32_t w[16];
+            decode32<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, h, w);
+            uint8_t* a = sa + ab * L::a_bytes + r * 128;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(a + (((4 * h + j) ^ (r & 7)) << 4)) =
+                    make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[ab]);
+            s += 2;
+            if (s >= kStages) {
+                s -= kStages;
+                ph ^= 1u;
+            }
+            ab += 2;
+            if (ab >= kABuffers) {
+                ab -= kABuffers;
+                ab_ph ^= 1u;
+            }
+        }
+    } else {
+        const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
+        const int mine = quarter * 32 + lane;
+        const bool f16 = p.y_type == SAMQ_TYPE_F16;
+        int acc = 0;
+        uint32_t acc_ph = 0, part_ph = 0;
+        for (int unit = cluster; unit < units; unit += clusters) {
+            const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
+            // This lane's weight row as a column of the group's output.
+            const int64_t col64 = static_cast<int64_t>(u.tile) * 128 + mine - static_cast<int64_t>(u.group) * p.n;
+            const bool in = col64 >= 0 && col64 < p.n;
+            const int col = static_cast<int>(col64);
+            const float bias = in && p.bias ? __ldg(p.bias + static_cast<int64_t>(u.group) * p.n + col) : 0.0f;
+            auto finish = [&](int t, float v) {
+                const int64_t row = u.row0 + t;
+                v += bias;
+                if (p.ids) {
+                    const int a = __ldg(p.ids + row);
+                    if (a >= 0 && a < p.adapter_count && in) {
+                        const uint4* b = reinterpret_cast<const uint4*>(p.b2 + (static_cast<int64_t>(a) * p.n + col) * 2 * p.rank);
+                        const uint4* hp = reinterpret_cast<const uint4*>(p.h2 + row * 2 * p.rank);
+                        const int words = p.rank / 8;
+                        float delta = 0.0f;
+#pragma unroll 2
+                        for (int j = 0; j < words; ++j) {
+                            const uint4 bv = __ldg(b + j), hv = __ldg(hp + j), lv = __ldg(hp + words + j);
+                            const __half2* b2 = reinterpret_cast<const __half2*>(&bv);
+                            const __half2* h2 = reinterpret_cast<const __half2*>(&hv);
+                            const __half2* l2 = reinterpret_cast<const __half2*>(&lv);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 x = __half22float2(b2[i]), y = __half22float2(h2[i]), z = __half22float2(l2[i]);
+                                delta = fmaf(y.x + z.x, x.x, delta);
+                                delta = fmaf(y.y + z.y, x.y, delta);
+                            }
+                        }
+                        v += delta;
+                    }
+                }
+                if (p.gelu) v = gelu_erf(v);
+                if (!in) return;
+                if (f16) static_cast<__half*>(p.y)[row * p.ldy + col] = __float2half_rn(v);
+                else static_cast<float*>(p.y)[row * p.ldy + col] = v;
+            };
+            // Warp-uniform: the TMEM loads below are warp-collective.
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 79))) break;
+            tc_fence_after();
+            const uint32_t d = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * TOK);
+            constexpr int C = TOK < 32 ? TOK : 32;
+            if (split > 1 &&
+                !__all_sync(0xffffffffu, mbar_wait_cluster(part_free, part_ph ^ 1u, status, 80)))
+                break;
+#pragma unroll 1
+            for (int c = 0; c < u.count; c += C) {
+                uint32_t v[C];
+                if constexpr (C == 16) tc_ld_32x32b_x16(d + c, v);
+                else tc_ld_32x32b_x32(d + c, v);
+                tc_wait_ld();
+                if (split > 1) {
+#pragma unroll
+                    for (int i = 0; i < C; ++i) spart[(c + i) * 128 + mine] = __uint_as_float(v[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < C; ++i)
+                        if (c + i < u.count) finish(c + i, __uint_as_float(v[i]));
+                }
+                __syncwarp();  // converged for the next collective load
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1u;
+            if (split > 1) {
+                if (lane < split) mbar_arrive_cluster(cluster_map(part_full, lane));
+                if (!__all_sync(0xffffffffu, mbar_wait_cluster(part_full, part_ph, status, 81))) break;
+                const uint32_t own = smem_u32(spart + mine);
+                for (int t = rank; t < u.count; t += split) {
+                    float v = 0.0f;
+                    for (int o = 0; o < split; ++o) {
+                        uint32_t remote;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(own + t * 512), "r"(o));
+                        v += ld_cluster(remote);
+                    }
+                    finish(t, v);
+                }
+                __syncwarp();
+                if (lane < split) mbar_arrive_cluster(cluster_map(part_free, lane));
+                part_ph ^= 1u;
+            }
+        }
+        tc_fence_before();
+    }
+    __syncwarp();
+    // A cluster: nobody reads this CTA's shared memory any more.
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// How many clusters of `split` CTAs of `kernel` can be resident on the device;
+// queried once per (kernel, device, split).
+int resident_clusters(DeviceState& state, const void* kernel, int split, int smem) {
+    static std::mutex mutex;
+    static std::map<std::tuple<const void*, int, int>, int> cache;
+    std::lock_guard<std::mutex> lock(mutex);
+    int& clusters = cache[{kernel, state.device, split}];
+    if (clusters > 0) return clusters;
+    DeviceGuard guard(state.device);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    check_cuda(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg), "cudaOccupancyMaxActiveClusters(routed rows)");
+    if (clusters <= 0) fail(SAMQ_ERR_CUDA, "no cluster of the routed rows kernel fits on this device");
+    return clusters;
+}
+
+template <int TYPE, int TOK>
+void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream) {
+    using L = RowsSmem<TYPE, TOK>;
+    CUtensorMap map;
+    encode_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, p.k, p.x_rows, p.ldx * 2, 64,
+                         p.row_index ? 1 : TOK, CU_TENSOR_MAP_SWIZZLE_128B);
+    auto kernel = routed_rows_kernel<TYPE, TOK>;
+    set_smem_limit_once(state, reinterpret_cast<const void*>(kernel), L::total,
+                        "cudaFuncSetAttribute(routed rows smem)");
+    const int tiles = (p.n + 127) / 128 + (p.n % 128 ? 1 : 0);  // of a group, at most
+    const int64_t units = std::min<int64_t>(p.rows, p.groups + p.rows / TOK) * tiles;  // at most
+    const int chunks = (p.k + 63) / 64;
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    // Few units: the widest cluster that still has every unit resident and leaves a CTA two steps or more.
+    int split = 1;
+    for (int wide = 2; wide <= kMaxSplit && chunks >= 2 * wide; wide *= 2) {
+        const bool all_work = (wide - 1) * ((chunks + wide - 1) / wide) < chunks;  // no rank without steps
+        if (all_work && units <= resident_clusters(state, fn, wide, L::total)) split = wide;
+    }
+    const int64_t clusters = std::min<int64_t>(units, split > 1 ? resident_clusters(state, fn, split, L::total) : state.sm_count);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = L::total;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    check_cuda(cudaLaunchKernelEx(&cfg, kernel, map, p, max_rows, split, state.status), "routed_rows_kernel launch");
+}
+
+template <int TYPE>
+void run_type(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream) {
+    const int64_t mean = (p.rows + p.groups - 1) / p.groups;
+    if (mean <= 16) run_rows<TYPE, 16>(p, max_rows, state, stream);
+    else if (mean <= 32) run_rows<TYPE, 32>(p, max_rows, state, stream);
+    else run_rows<TYPE, 64>(p, max_rows, state, stream);
+}
+
+}  // namespace
+
+void launch_routed_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream) {
+    switch (p.type) {
+        case SAMQ_TYPE_Q8_0: run_type<SAMQ_TYPE_Q8_0>(p, max_rows, state, stream); break;
+        case SAMQ_TYPE_Q4_K: run_type<SAMQ_TYPE_Q4_K>(p, max_rows, state, stream); break;
+        case SAMQ_TYPE_Q5_K: run_type<SAMQ_TYPE_Q5_K>(p, max_rows, state, stream); break;
+        default: run_type<SAMQ_TYPE_Q6_K>(p, max_rows, state, stream); break;
+    }
+}
+
+}  // namespace samq

@@ -452,6 +452,8 @@ void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, 
                          cudaStream_t stream);
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
 constexpr int kRoutedFewRows = 64;  // rows of a group, at most, that take the packet-streaming kernel
+// routed_rows.cu: the groups of at most `max_rows` rows from their packets.
+void launch_routed_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream);
 // routed_tile.cu: the groups of at least `min_rows` rows on tensor-core tiles.
 void launch_routed_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream);
 

@@ -287,6 +287,27 @@ def test_grouped_one_group_is_the_plain_linear(samq, oracle):
     w.close()
 
 
+@pytest.mark.parametrize("qtype,k", [(Q8_0, 96), (Q8_0, 320), (Q4_K, 512), (Q5_K, 512), (Q6_K, 512)])
+@pytest.mark.parametrize("n,groups", [(128, 2), (200, 3), (40, 7)])
+def test_grouped_decodes_every_weight(samq, oracle, qtype, k, n, groups):
+    """Unit vectors as activations read the weight operand back, bit for bit, whichever kernel multiplies."""
+    rng = np.random.default_rng(k + n)
+    gguf, w64 = packed(oracle, rng, qtype, groups * n, k)
+    weights = samq.Weights(qtype, k, groups * n, gguf)
+    for rows_each in (4, 100):
+        rows = rows_each * groups
+        for base in range(0, k, rows_each):
+            cols = (base + np.arange(rows)) % k
+            x = np.zeros((rows, k), H)
+            x[np.arange(rows), cols] = 1
+            y = torch.empty(rows, (n + 3) // 4 * 4, device="cuda")
+            samq.linear_grouped(weights, groups, dev(x), rows, k, dev(np.arange(groups + 1, dtype=np.int32) * rows_each),
+                                rows, y, y.shape[1])
+            want = np.stack([w64[(i // rows_each) * n:(i // rows_each + 1) * n, cols[i]] for i in range(rows)])
+            np.testing.assert_array_equal(host(y)[:, :n], want.astype(F))
+    weights.close()
+
+
 # ---- combine --------------------------------------------------------------------
 
 @pytest.mark.parametrize("tokens,top_k,width,dtype,residual,in_place", [
