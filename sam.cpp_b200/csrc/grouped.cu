@@ -1,8 +1,8 @@
 // grouped.cu -- products whose weight depends on the row (samq_linear_grouped_v1,
 // samq_linear_adapters_v1): y[i] = act(W_g x[row_index[i]] + bias_g + delta_i)
 // for the rows i of group g, with delta the row's low-rank adapter.  Here the
-// operand in plan order, the adapters' down product and the choice of kernel;
-// the products themselves are in routed_rows.cu and routed_tile.cu.
+// operand in plan order and the choice of kernel; the products themselves are in
+// routed_rows.cu and routed_tile.cu, the adapters' down product in adapters.cu.
 #include <algorithm>
 #include <climits>
 
@@ -10,36 +10,6 @@
 
 namespace samq {
 namespace {
-
-// h2[i] = hi | lo of scale_a A_a x[i]: one warp per (row, rank index).
-__global__ void __launch_bounds__(256) adapter_down_kernel(const RoutedProduct p, const __half* __restrict__ a_all,
-                                                           const float* __restrict__ scales,
-                                                           const int* __restrict__ ranks, __half* __restrict__ h2,
-                                                           DeviceStatus* status) {
-    pdl_wait();
-    pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int64_t task = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int64_t row = task / p.rank;
-    const int r = static_cast<int>(task - row * p.rank);
-    if (row >= p.rows) return;
-    const int a = p.ids[row];
-    float v = 0.0f;
-    if (a >= 0 && a < p.adapter_count && r < ranks[a]) {
-        const __half* av = a_all + (static_cast<int64_t>(a) * p.rank + r) * p.k;
-        for (int c = lane; c < p.k; c += 32)
-            v = fmaf(__half2float(p.x[row * p.ldx + c]), __half2float(av[c]), v);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        v *= scales[a];
-    }
-    record_range(!(fabsf(v) <= kOperandLimit), status);
-    if (lane == 0) {
-        const __half hi = __float2half_rn(v);
-        h2[row * 2 * p.rank + r] = hi;
-        h2[row * 2 * p.rank + p.rank + r] = __float2half_rn(v - __half2float(hi));
-    }
-}
 
 // The product's operand in plan order, f16 [rows][k]: row i is x[row_index[i]]
 // (zeros for an index outside [0, x_rows)), f32 rows staged by the Q8_1 rule on
@@ -92,14 +62,6 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
     else
         launch_pdl(gather_rows_kernel<float>, grid, dim3(256), 0, stream, "gather_rows_kernel launch",
                    static_cast<const float*>(x), x_rows, ldx, row_index, rows, k, out, state.status);
-}
-
-void launch_adapter_down(const RoutedProduct& p, const samq_adapters& ad, __half* h2, DeviceState& state,
-                         cudaStream_t stream) {
-    const int64_t warps = p.rows * ad.rank;
-    launch_pdl(adapter_down_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream,
-               "adapter_down_kernel launch", p, static_cast<const __half*>(ad.a), static_cast<const float*>(ad.scale),
-               static_cast<const int*>(ad.ranks), h2, state.status);
 }
 
 // Few rows stream the packets, many take the f16 tiles.  Between, a call holds
