@@ -18,8 +18,11 @@
 //   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
 //                shared memory and back, summed over the cluster), bias, adapters,
 //                erf-GELU, stores coalesced over the weight rows;
-//   warps 6-21   decoders, two sets of eight on alternate steps: a thread turns 32
-//                columns of a row into f16 with the values of packets.cuh bit for bit.
+//   warps 6-21   decoders, four sets of four on steps in turn: a thread turns a row
+//                of its packet into f16 with the values of packets.cuh bit for bit and
+//                stores it to tensor memory, where the MMA takes it as its left
+//                factor (through shared memory, with the fence that needs, a step cost
+//                925 cycles instead of @@ at Q4_K).
 // The decoders are the busiest pipe, hence their arithmetic: a nibble becomes a
 // float by or-ing it into the mantissa of 2^23 where it stands (the sub-block's
 // scale takes the power of 16), and pairs of weights share packed f32 operations;
@@ -39,7 +42,8 @@ namespace {
 
 constexpr int kDecodeWarps = 16;
 constexpr int kThreads = 32 * (6 + kDecodeWarps);
-constexpr int kABuffers = 4;
+constexpr int kSets = kDecodeWarps / 4;
+constexpr int kABuffers = 2 * kSets;  // of 32 TMEM columns: 128 rows x 64 f16
 constexpr int kMaxGroups = 1024;
 constexpr int kSmemLimit = 232448;
 constexpr int kMaxSplit = 8;
@@ -48,15 +52,13 @@ template <int TYPE, int TOK>
 struct RowsSmem {
     static constexpr int raw_bytes = 128 * (code_bytes_of(TYPE) + 8);  // one packet
     static constexpr int x_bytes = TOK * 128;
-    static constexpr int a_bytes = 128 * 128;
     static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
     static constexpr int tables = (3 * kMaxGroups + 1) * 4;
-    static constexpr int fixed = 1024 + kABuffers * a_bytes + part + 512 + tables;
-    static constexpr int stages = (kSmemLimit - fixed) / (raw_bytes + x_bytes) > 12
-                                      ? 12
+    static constexpr int fixed = 1024 + part + 512 + tables;
+    static constexpr int stages = (kSmemLimit - fixed) / (raw_bytes + x_bytes) > 16
+                                      ? 16
                                       : (kSmemLimit - fixed) / (raw_bytes + x_bytes);
-    static constexpr int x_off = kABuffers * a_bytes;
-    static constexpr int raw_off = x_off + stages * x_bytes;
+    static constexpr int raw_off = stages * x_bytes;
     static constexpr int part_off = raw_off + stages * raw_bytes;
     static constexpr int bar_off = part_off + part;
     static constexpr int table_off = bar_off + 512;
@@ -89,23 +91,21 @@ __device__ __forceinline__ uint32_t half2_of(uint64_t v) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float half_at(const uint8_t* p) {
-    return __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(p)));
-}
-
-// Columns 32 h .. 32 h + 31 of a packet row as f16: word i of `out` holds columns
-// 2 i and 2 i + 1 of the 32.
+// A packet row (codes `code`, scale record `rec`) as f16: word i of `out` holds
+// columns 2 i and 2 i + 1 of the 64.
 template <int TYPE>
-__device__ __forceinline__ void decode32(const uint8_t* __restrict__ code, const uint8_t* __restrict__ rec, int h,
-                                         uint32_t (&out)[16]) {
+__device__ __forceinline__ void decode_row(const uint8_t* __restrict__ code, const uint8_t* __restrict__ rec,
+                                           uint32_t (&out)[32]) {
+    const uint2 record = *reinterpret_cast<const uint2*>(rec);
     if constexpr (TYPE == SAMQ_TYPE_Q8_0) {
-        const __half2 d = __half2half2(__ushort_as_half(*reinterpret_cast<const uint16_t*>(rec + 2 * h)));
         const __half2 bias = __floats2half2_rn(-1152.0f, -1152.0f);  // 1024 of the mantissa trick, 128 of the sign
-        uint32_t w[8];
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(code + 32 * h);
-        *reinterpret_cast<uint4*>(w + 4) = *reinterpret_cast<const uint4*>(code + 32 * h + 16);
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(code + 16 * i);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const __half2 d = __half2half2(__ushort_as_half(static_cast<uint16_t>(i < 8 ? record.x : record.x >> 16)));
             const uint32_t u = w[i] ^ 0x80808080u;
             const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
             const __half2 a = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&lo), bias), d);
@@ -115,26 +115,30 @@ __device__ __forceinline__ void decode32(const uint8_t* __restrict__ code, const
         }
     } else {
         // Words of 8 nibbles (column 8 j + i at bit 4 i).
-        uint32_t lo[4];
+        uint32_t lo[8];
         if constexpr (TYPE == SAMQ_TYPE_Q5_K) {  // 40-byte rows
-            *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(code + 16 * h);
-            *reinterpret_cast<uint2*>(lo + 2) = *reinterpret_cast<const uint2*>(code + 16 * h + 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2*>(lo + 2 * i) = *reinterpret_cast<const uint2*>(code + 8 * i);
         } else {
-            *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(code + 16 * h);
+            *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(code);
+            *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(code + 16);
         }
         // Column i of a word's lower (upper, shifted down) half stands at bit 4 (i % 4): worth 16^(i % 4) in the
         // mantissa of 2^23, where up to 23 bits are free.
         constexpr uint32_t kMagic = 0x4b000000u;
-        const float d = half_at(rec);
+        const float d = __half2float(__ushort_as_half(static_cast<uint16_t>(record.x)));
         if constexpr (TYPE == SAMQ_TYPE_Q6_K) {
-            const uint2 hi = *reinterpret_cast<const uint2*>(code + 32 + 8 * h);  // 2 bits a column
+            uint32_t high[4];  // 2 bits a column
+            *reinterpret_cast<uint4*>(high) = *reinterpret_cast<const uint4*>(code + 32);
             const uint64_t off01 = pack2(-8388608.0f - 32.0f, -8388608.0f - 512.0f);
             const uint64_t off23 = pack2(-8388608.0f - 8192.0f, -8388608.0f - 131072.0f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float ds = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(rec[2 + 2 * h + (j >> 1)])));
+            for (int j = 0; j < 8; ++j) {
+                const int sc = static_cast<int8_t>((j < 4 ? record.x >> (16 + 8 * (j >> 1)) : record.y >> (8 * ((j >> 1) - 2))) & 0xffu);
+                const float ds = __fmul_rn(d, static_cast<float>(sc));
                 const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
-                const uint32_t bits = ((j & 2) ? hi.y : hi.x) >> (16 * (j & 1));
+                const uint32_t bits = high[j >> 1] >> (16 * (j & 1));
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     const uint32_t n = lo[j] >> (16 * q), b = (bits >> (8 * q)) & 0xffu;
@@ -149,31 +153,36 @@ __device__ __forceinline__ void decode32(const uint8_t* __restrict__ code, const
                 }
             }
         } else {
-            const float ds = __fmul_rn(d, static_cast<float>(rec[4 + h]));
-            const float dm = __fmul_rn(half_at(rec + 2), static_cast<float>(rec[6 + h]));
-            const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
-            const uint64_t m2 = pack2(-dm, -dm), off = pack2(-8388608.0f, -8388608.0f);
-            uint32_t high = 0;
-            if constexpr (TYPE == SAMQ_TYPE_Q5_K) high = *reinterpret_cast<const uint32_t*>(code + 32 + 4 * h);
+            const float dmin = __half2float(__ushort_as_half(static_cast<uint16_t>(record.x >> 16)));
+            const uint64_t off = pack2(-8388608.0f, -8388608.0f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int h = 0; h < 2; ++h) {
+                const float ds = __fmul_rn(d, static_cast<float>((record.y >> (8 * h)) & 0xffu));
+                const float dm = __fmul_rn(dmin, static_cast<float>((record.y >> (16 + 8 * h)) & 0xffu));
+                const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
+                const uint64_t m2 = pack2(-dm, -dm);
+                uint32_t high = 0;
+                if constexpr (TYPE == SAMQ_TYPE_Q5_K) high = *reinterpret_cast<const uint32_t*>(code + 32 + 4 * h);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t n = lo[j] >> (16 * q);
-                    uint32_t v0 = (n & 0xfu) | kMagic, v1 = (n & 0xf0u) | kMagic;
-                    uint32_t v2 = (n & 0xf00u) | kMagic, v3 = (n & 0xf000u) | kMagic;
-                    if constexpr (TYPE == SAMQ_TYPE_Q5_K) {
-                        const uint32_t b = high >> (8 * j + 4 * q);
-                        v0 |= (b << 4) & 0x10u;
-                        v1 |= (b << 7) & 0x100u;
-                        v2 |= (b << 10) & 0x1000u;
-                        v3 |= (b << 13) & 0x10000u;
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t n = lo[4 * h + j] >> (16 * q);
+                        uint32_t v0 = (n & 0xfu) | kMagic, v1 = (n & 0xf0u) | kMagic;
+                        uint32_t v2 = (n & 0xf00u) | kMagic, v3 = (n & 0xf000u) | kMagic;
+                        if constexpr (TYPE == SAMQ_TYPE_Q5_K) {
+                            const uint32_t b = high >> (8 * j + 4 * q);
+                            v0 |= (b << 4) & 0x10u;
+                            v1 |= (b << 7) & 0x100u;
+                            v2 |= (b << 10) & 0x1000u;
+                            v3 |= (b << 13) & 0x10000u;
+                        }
+                        // ds q has at most 22 bits, so the fused form rounds where the separate one does
+                        out[16 * h + 4 * j + 2 * q] =
+                            half2_of(fma2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off), s01, m2));
+                        out[16 * h + 4 * j + 2 * q + 1] =
+                            half2_of(fma2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off), s23, m2));
                     }
-                    // ds q has at most 22 bits, so the fused form rounds where the separate one does
-                    out[4 * j + 2 * q] =
-                        half2_of(fma2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off), s01, m2));
-                    out[4 * j + 2 * q + 1] =
-                        half2_of(fma2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off), s23, m2));
                 }
             }
         }
@@ -232,11 +241,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                    DeviceStatus* status) {
     using L = RowsSmem<TYPE, TOK>;
     constexpr int kStages = L::stages;
-    static_assert(kStages >= 4 && L::total <= kSmemLimit, "shared memory budget");
+    static_assert(kStages >= kSets && L::total <= kSmemLimit, "shared memory budget");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sa = smem;
-    uint8_t* sx = smem + L::x_off;
+    uint8_t* sx = smem;
     uint8_t* sraw = smem + L::raw_off;
     float* spart = reinterpret_cast<float*>(smem + L::part_off);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
@@ -260,7 +268,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     const int chunks = (p.k + 63) / 64;
     const int per = (chunks + split - 1) / split;  // steps of a rank (the host leaves none without)
     const int c_begin = rank * per, steps = min(chunks, c_begin + per) - c_begin;
-    constexpr uint32_t kTmemCols = 2 * TOK;
+    constexpr uint32_t kTmemCols = 512;           // 2 x TOK accumulator columns, then the left factors
+    constexpr uint32_t kTmemA = 2 * TOK;
+    static_assert(2 * TOK + 32 * kABuffers <= 512, "tensor memory");
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -268,7 +278,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < kABuffers; ++b) {
-            mbar_init(&a_full[b], kDecodeWarps / 2);
+            mbar_init(&a_full[b], 4);
             mbar_init(&a_empty[b], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -365,7 +375,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_f16_f32(128, TOK);
-            const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), x_desc = smem_desc_sw128(smem_u32(sx));
+            const uint64_t x_desc = smem_desc_sw128(smem_u32(sx));
             int s = 0, ab = 0, acc = 0;
             uint32_t ph = 0, ab_ph = 0, acc_ph = 0;
             bool ok = true;
@@ -379,11 +389,11 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t ad = a_desc + static_cast<uint32_t>(ab * (L::a_bytes >> 4));
+                    const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(ab * 32);
                     const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        tc_mma_f16(d, ad + 2 * kk, xd + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
+                        tc_mma_f16_ts(d, a + 8 * kk, xd + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
                     tc_commit(&empty[s]);
                     tc_commit(&a_empty[ab]);
                     if (++s == kStages) {
@@ -405,34 +415,33 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
         }
         __syncwarp();
     } else if (warp >= 6) {
-        // Step q of the CTA (over all its units) goes to set q & 1, buffer q % kABuffers.
-        const int set = (warp - 6) >> 3;
-        const int id = ((warp - 6) & 7) * 32 + lane;
-        const int r = id >> 1, h = id & 1;
-        int s = set, ab = set;  // stage and buffer of this set's next step (kStages >= 2)
+        // Step q of the CTA (over all its units) goes to set q % kSets, buffer q % kABuffers.
+        const int set = (warp - 6) >> 2;
+        const int quarter = warp & 3;  // the TMEM lanes a warp may store to
+        const int r = quarter * 32 + lane;
+        const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemA;
+        int s = set % kStages, ab = set;  // stage and buffer of this set's next step
         uint32_t ph = 0, ab_ph = 0;
         const int my_units = units > cluster ? (units - cluster + clusters - 1) / clusters : 0;
         const int total = my_units * steps;
-        for (int q = set; q < total; q += 2) {
-            const bool ok = mbar_wait(&full[s], ph, status, 77) && mbar_wait(&a_empty[ab], ab_ph ^ 1u, status, 78);
-            if (!__all_sync(0xffffffffu, ok)) break;
+        for (int q = set; q < total; q += kSets) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, status, 77))) break;
             const uint8_t* raw = sraw + s * L::raw_bytes;
-            uint32_t w[16];
-            decode32<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, h, w);
-            uint8_t* a = sa + ab * L::a_bytes + r * 128;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4*>(a + (((4 * h + j) ^ (r & 7)) << 4)) =
-                    make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-            fence_proxy_async_smem();
+            uint32_t w[32];
+            decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, w);
+            if (!__all_sync(0xffffffffu, mbar_wait(&a_empty[ab], ab_ph ^ 1u, status, 78))) break;
+            tc_fence_after();
+            tc_st_32x32b_x32(lanes + static_cast<uint32_t>(ab * 32), w);
+            tc_wait_st();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[ab]);
-            s += 2;
+            s += kSets;
             if (s >= kStages) {
                 s -= kStages;
                 ph ^= 1u;
             }
-            ab += 2;
+            ab += kSets;
             if (ab >= kABuffers) {
                 ab -= kABuffers;
                 ab_ph ^= 1u;

@@ -20,10 +20,12 @@
 //
 // Pipeline (one CTA or CTA pair per SM or TPC, persistent over the tiles of all
 // groups):
-//   warp 0     producer: 128 x 64 of X and BN (a pair: BN / 2 each) x 64 of W per
-//              step by TMA, 128-byte swizzle, kStages deep.  Each step's `last`
-//              flag travels with its stage, as only the producer knows how many
-//              adapters a tile has;
+//   warp 0     W producer: BN (a pair: BN / 2 each) x 64 of W per step by TMA,
+//              128-byte swizzle, kStages deep;
+//   last warp  X producer: 128 x 64 of X.  Each step's `last` flag travels with its
+//              stage, as only the producers know how many adapters a tile has.  Two
+//              warps as a step's wait, announcement and two copies take one thread
+//              longer than the tensor cores need for it (512 cycles);
 //   warp 1     TMEM owner; one thread (of the even CTA) issues tcgen05.mma;
 //   warps 2..  epilogue: accumulator out of TMEM, bias, erf-GELU, 32 rows of 128
 //              bytes at a time through swizzled shared memory: one TMA store, or,
@@ -41,7 +43,8 @@ constexpr int BM = 128;  // rows of a CTA's tile
 constexpr int BK = 64;   // depth of a step: one 128-byte swizzle row of f16
 constexpr int kAccStride = 256;
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kThreads = 96 + 32 * kEpilogueWarps;
+constexpr int kXWarp = 2 + kEpilogueWarps;
 constexpr int kSlabBytes = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int kSmemLimit = 232448;
 
@@ -203,21 +206,23 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
     const uint32_t tmem_base = *tmem_slot;
     const int tiles = s_first[p.groups] * n_tiles;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == kXWarp) {
+        // Both producers walk the same steps; the X warp announces them.
+        const bool is_x = warp == kXWarp;
         int s = 0;
         uint32_t ph = 0;
         uint32_t issued = 0, issued_phase = 0;
         bool ok = true;
         const int no_row = static_cast<int>(p.rows);  // an index that reads zeros
         const uint32_t full_bar = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);  // the even CTA's
-        // Lane 0: waits for the next stage, announces the step and loads B from `bm`.
-        auto open = [&](const CUtensorMap* bm, int brow, int x, bool last) -> bool {
+        const int b_half = rank * (BN / CTAS);
+        // Lane 0: waits for the next stage; the X warp announces the step.
+        auto open = [&](bool last) -> bool {
             if (!mbar_wait(&empty[s], ph ^ 1u, status, 61)) return false;
-            if (rank == 0) {
+            if (is_x && rank == 0) {
                 last_step[s] = last;
                 mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
             }
-            tma_tile<CTAS>(sb + s * L::b_bytes, bm, &full[s], full_bar + 8 * s, x, brow + rank * (BN / CTAS));
             issued |= 1u << s;
             issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
             return true;
@@ -247,12 +252,15 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 next = __reduce_min_sync(0xffffffffu, next);
             }
             if (lane == 0) {
-                const int wrow = t.group * p.n + t.col0;
+                const int wrow = t.group * p.n + t.col0 + b_half;
                 const bool plain = next >= p.adapter_count;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    ok = open(&maps.w, wrow, kb * BK, kb == kblocks - 1 && plain);
+                    ok = open(kb == kblocks - 1 && plain);
                     if (!ok) break;
-                    tma_tile<CTAS>(sa + s * L::a_bytes, &maps.x, &full[s], full_bar + 8 * s, kb * BK, row0);
+                    if (is_x)
+                        tma_tile<CTAS>(sa + s * L::a_bytes, &maps.x, &full[s], full_bar + 8 * s, kb * BK, row0);
+                    else
+                        tma_tile<CTAS>(sb + s * L::b_bytes, &maps.w, &full[s], full_bar + 8 * s, kb * BK, wrow);
                     advance();
                 }
             }
@@ -275,13 +283,16 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 const int4 rows4 = make_int4(v[0], v[1], v[2], v[3]);
                 for (int c = 0; c < 2 * p.rank && ok; c += BK) {
                     if (lane == 0) {
-                        ok = open(&maps.b, a * p.n + t.col0, c, c + BK >= 2 * p.rank && next >= p.adapter_count);
-                        if (ok && all)
+                        ok = open(c + BK >= 2 * p.rank && next >= p.adapter_count);
+                        if (ok && !is_x)
+                            tma_tile<CTAS>(sb + s * L::b_bytes, &maps.b, &full[s], full_bar + 8 * s, c,
+                                           a * p.n + t.col0 + b_half);
+                        else if (ok && all)
                             tma_tile<CTAS>(sa + s * L::a_bytes, &maps.h, &full[s], full_bar + 8 * s, c, row0);
                     }
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     const int stage = __shfl_sync(0xffffffffu, s, 0);
-                    if (ok && !all)
+                    if (ok && is_x && !all)
                         tma_gather4<CTAS>(sa + stage * L::a_bytes + lane * 512, &maps.h_rows, full_bar + 8 * stage, c,
                                           rows4);
                     if (lane == 0 && ok) advance();
@@ -307,6 +318,13 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), b_desc = smem_desc_sw128(smem_u32(sb));
             int s = 0;
             uint32_t ph = 0;
+            auto wait_full = [&](int i, uint32_t phase) {
+                return CTAS == 2 ? mbar_wait_cluster(&full[i], phase, status, 63) : mbar_wait(&full[i], phase, status, 63);
+            };
+            auto probe_full = [&](int i, uint32_t phase) {
+                return CTAS == 2 ? mbar_test_wait_cluster(&full[i], phase) : mbar_test_wait(&full[i], phase);
+            };
+            bool ready = false;
             int acc = 0;
             uint32_t acc_ph = 0;
             bool ok = true;
@@ -319,9 +337,8 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 uint32_t accumulate = 0;
                 bool last = false;
                 while (!last) {
-                    const bool filled = CTAS == 2 ? mbar_wait_cluster(&full[s], ph, status, 63)
-                                                  : mbar_wait(&full[s], ph, status, 63);
-                    if (!filled) {
+                    // The probe of this stage was issued under the previous step's MMAs.
+                    if (!ready && !wait_full(s, ph)) {
                         ok = false;
                         break;
                     }
@@ -329,18 +346,20 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                     last = last_step[s] != 0;
                     const uint64_t ad = a_desc + static_cast<uint32_t>(s * (L::a_bytes >> 4));
                     const uint64_t bd = b_desc + static_cast<uint32_t>(s * (L::b_bytes >> 4));
+                    const int now = s;
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                    ready = probe_full(s, ph);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk) {
                         if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
                         else tc_mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
                         accumulate = 1;
                     }
-                    if constexpr (CTAS == 2) tc_commit_both(&empty[s]);
-                    else tc_commit(&empty[s]);
-                    if (++s == kStages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
+                    if constexpr (CTAS == 2) tc_commit_both(&empty[now]);
+                    else tc_commit(&empty[now]);
                 }
                 if (!ok) break;
                 if constexpr (CTAS == 2) tc_commit_both(&tfull[acc]);
