@@ -12,22 +12,24 @@
 // one launch, no atomics, no workspace.
 //
 // One CTA per SM, persistent over the units of all groups:
-//   warp 0       each step's packet by a bulk copy, its 64 columns of X by TMA (rows
-//                by index through the row gather), kStages deep;
+//   warp 0       each step's packets (kDepth of them, contiguous) by one bulk copy;
+//   last warp    the same columns of X by TMA (rows by index through the row gather);
 //   warp 1       TMEM owner; one thread issues the MMAs;
 //   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
 //                shared memory and back, summed over the cluster), bias, adapters,
 //                erf-GELU, stores coalesced over the weight rows;
-//   warps 6-21   decoders, four sets of four on steps in turn: a thread turns a row
-//                of its packet into f16 with the values of packets.cuh bit for bit and
-//                stores it to tensor memory, where the MMA takes it as its left
-//                factor (through shared memory, with the fence that needs, a step cost
-//                925 cycles instead of @@ at Q4_K).
-// The decoders are the busiest pipe, hence their arithmetic: a nibble becomes a
-// float by or-ing it into the mantissa of 2^23 where it stands (the sub-block's
-// scale takes the power of 16), and pairs of weights share packed f32 operations;
-// an int8 becomes a half by the same trick with 1024, and f16(q d) needs a
-// single half multiplication as q d has at most 19 bits.
+//   warps 6-     decoders, sets of four on steps in turn: a thread turns a row of its
+//                packets into f16 with the values of packets.cuh bit for bit and stores
+//                it to tensor memory, where the MMA takes it as its left factor.
+// A step costs the thread that issues its copies about 250 cycles and the MMA
+// thread as much whatever its size, while a Q4_K packet takes 210 cycles of HBM
+// bandwidth: hence kDepth packets a step, one thread per kind of copy, and one
+// barrier pair for a step's shared and tensor memory.
+// The decoders' arithmetic: a nibble becomes a float by or-ing it into the
+// mantissa of 2^23 where it stands (the sub-block's scale takes the power of 16),
+// and pairs of weights share packed f32 operations; an int8 becomes a half by the
+// same trick with 1024, and f16(q d) needs a single half multiplication as q d has
+// at most 19 bits.
 // Every wait is bounded.  No load uses multicast.
 #include <algorithm>
 #include <climits>
@@ -41,27 +43,32 @@ namespace samq {
 namespace {
 
 constexpr int kDecodeWarps = 16;
-constexpr int kThreads = 32 * (6 + kDecodeWarps);
+constexpr int kXWarp = 6 + kDecodeWarps;
+constexpr int kThreads = 32 * (kXWarp + 1);
 constexpr int kSets = kDecodeWarps / 4;
-constexpr int kABuffers = 2 * kSets;  // of 32 TMEM columns: 128 rows x 64 f16
+constexpr int kDepth = 2;             // packets (64 columns each) of a step
+constexpr int kTmemStep = 32 * kDepth;  // TMEM columns of a step's left factor: 128 rows x 64 kDepth f16
 constexpr int kMaxGroups = 1024;
 constexpr int kSmemLimit = 232448;
 constexpr int kMaxSplit = 8;
 
 template <int TYPE, int TOK>
 struct RowsSmem {
-    static constexpr int raw_bytes = 128 * (code_bytes_of(TYPE) + 8);  // one packet
-    static constexpr int x_bytes = TOK * 128;
+    static constexpr int packet = 128 * (code_bytes_of(TYPE) + 8);
+    static constexpr int raw_bytes = kDepth * packet;
+    static constexpr int x_chunk = TOK * 128;  // 64 columns of TOK rows
+    static constexpr int x_bytes = kDepth * x_chunk;
     static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
     static constexpr int tables = (3 * kMaxGroups + 1) * 4;
-    static constexpr int fixed = 1024 + part + 512 + tables;
-    static constexpr int stages = (kSmemLimit - fixed) / (raw_bytes + x_bytes) > 16
-                                      ? 16
-                                      : (kSmemLimit - fixed) / (raw_bytes + x_bytes);
+    static constexpr int fixed = 1024 + part + 256 + tables;
+    // A stage is a step's packets and X in shared memory and its left factor in tensor memory.
+    static constexpr int by_smem = (kSmemLimit - fixed) / (raw_bytes + x_bytes);
+    static constexpr int by_tmem = (512 - 2 * TOK) / kTmemStep;
+    static constexpr int stages = by_smem < by_tmem ? by_smem : by_tmem;
     static constexpr int raw_off = stages * x_bytes;
     static constexpr int part_off = raw_off + stages * raw_bytes;
     static constexpr int bar_off = part_off + part;
-    static constexpr int table_off = bar_off + 512;
+    static constexpr int table_off = bar_off + 256;
     static constexpr int total = fixed + stages * (raw_bytes + x_bytes);
 };
 
@@ -250,14 +257,13 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
     uint64_t* empty = full + kStages;
     uint64_t* a_full = empty + kStages;
-    uint64_t* a_empty = a_full + kABuffers;
-    uint64_t* tfull = a_empty + kABuffers;
+    uint64_t* tfull = a_full + kStages;
     uint64_t* tempty = tfull + 2;
     uint64_t* part_full = tempty + 2;   // every CTA of the cluster has written its partial sums
     uint64_t* part_free = part_full + 1;  // every CTA has read this one's
     uint64_t* drain = part_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    static_assert((2 * kStages + 2 * kABuffers + 4 + 3) * 8 + 4 <= 512, "barrier space");
+    static_assert((3 * kStages + 4 + 3) * 8 + 4 <= 256, "barrier space");
     int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
     int* s_end = s_begin + kMaxGroups;
     int* s_first = s_end + kMaxGroups;
@@ -266,20 +272,17 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
     const int cluster = blockIdx.x / split, clusters = gridDim.x / split;
     const int chunks = (p.k + 63) / 64;
-    const int per = (chunks + split - 1) / split;  // steps of a rank (the host leaves none without)
-    const int c_begin = rank * per, steps = min(chunks, c_begin + per) - c_begin;
-    constexpr uint32_t kTmemCols = 512;           // 2 x TOK accumulator columns, then the left factors
+    const int all_steps = (chunks + kDepth - 1) / kDepth;
+    const int per = (all_steps + split - 1) / split;  // steps of a rank (the host leaves none without)
+    const int step0 = rank * per, steps = min(all_steps, step0 + per) - step0;
+    constexpr uint32_t kTmemCols = 512;  // 2 x TOK accumulator columns, then the left factors
     constexpr uint32_t kTmemA = 2 * TOK;
-    static_assert(2 * TOK + 32 * kABuffers <= 512, "tensor memory");
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 2);
             mbar_init(&empty[s], 1);
-        }
-        for (int b = 0; b < kABuffers; ++b) {
-            mbar_init(&a_full[b], 4);
-            mbar_init(&a_empty[b], 1);
+            mbar_init(&a_full[s], 4);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
@@ -324,85 +327,101 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     const uint32_t tmem_base = *tmem_slot;
     const int units = s_first[p.groups];
 
-    if (warp == 0) {
+    if (warp == 0 || warp == kXWarp) {
+        const bool is_x = warp == kXWarp;
         int s = 0;
         uint32_t ph = 0;
         uint32_t issued = 0, issued_phase = 0;
         bool ok = true;
-        for (int unit = cluster; unit < units && ok; unit += clusters) {
-            const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
-            const uint8_t* packet = p.packets + (static_cast<int64_t>(u.tile) * chunks + c_begin) * L::raw_bytes;
-            int rows[4];
-            if (p.row_index && lane < TOK / 4) {
+        auto advance = [&] {
+            issued |= 1u << s;
+            issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
+            if (++s == kStages) {
+                s = 0;
+                ph ^= 1u;
+            }
+        };
+        if (is_x && p.row_index) {
+            for (int unit = cluster; unit < units && ok; unit += clusters) {
+                const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
+                int rows[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 4 * lane + j < u.count ? __ldg(p.row_index + u.row0 + 4 * lane + j) : -1;
                     rows[j] = r >= 0 && r < p.x_rows ? r : static_cast<int>(p.x_rows);  // past the end: zeros
                 }
+                for (int i = step0; i < step0 + steps; ++i) {
+                    const int here = min(kDepth, chunks - i * kDepth);  // packets of this step
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 71));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                    __syncwarp();
+                    if (lane < TOK / 4)
+                        for (int c = 0; c < here; ++c)
+                            gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
+                                    (i * kDepth + c) * 64, rows);
+                    advance();
+                }
             }
-            for (int i = 0; i < steps && ok; ++i) {
-                if (lane == 0) {
+        } else if (elect_one()) {
+            for (int unit = cluster; unit < units && ok; unit += clusters) {
+                const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
+                const uint8_t* packet = p.packets + static_cast<int64_t>(u.tile) * chunks * L::packet;
+                for (int i = step0; i < step0 + steps; ++i) {
+                    const int here = min(kDepth, chunks - i * kDepth);
                     ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
-                    if (ok) {
-                        mbar_arrive_expect_tx(&full[s], L::raw_bytes + L::x_bytes);
+                    if (!ok) break;
+                    if (!is_x) {
+                        mbar_arrive_expect_tx(&full[s], here * L::packet);
                         bulk_load_1d(sraw + s * L::raw_bytes, packet + static_cast<int64_t>(i) * L::raw_bytes,
-                                     L::raw_bytes, &full[s]);
-                        if (!p.row_index)
-                            tma_load_2d(sx + s * L::x_bytes, &map_x, &full[s], (c_begin + i) * 64, u.row0);
+                                     here * L::packet, &full[s]);
+                    } else {
+                        mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                        for (int c = 0; c < here; ++c)
+                            tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s], (i * kDepth + c) * 64,
+                                        u.row0);
                     }
-                }
-                if (p.row_index) {
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (ok && lane < TOK / 4)
-                        gather4(sx + s * L::x_bytes + lane * 512, &map_x, &full[s], (c_begin + i) * 64, rows);
-                }
-                if (!ok) break;
-                issued |= 1u << s;
-                issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
-                if (++s == kStages) {
-                    s = 0;
-                    ph ^= 1u;
+                    advance();
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
         }
-        pdl_trigger();  // all loads issued
-        if (!ok && lane == 0) {  // let the copies in flight land before the CTA exits
+        pdl_trigger();  // this thread's loads are issued
+        if (!ok) {  // let the copies in flight land before the CTA exits
             for (int i = 0; i < kStages; ++i)
                 if (issued & (1u << i)) mbar_wait(&full[i], (issued_phase >> i) & 1u, status, 75);
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16_f32(128, TOK);
             const uint64_t x_desc = smem_desc_sw128(smem_u32(sx));
-            int s = 0, ab = 0, acc = 0;
-            uint32_t ph = 0, ab_ph = 0, acc_ph = 0;
+            int s = 0, acc = 0;
+            uint32_t ph = 0, acc_ph = 0;
             bool ok = true;
             for (int unit = cluster; unit < units && ok; unit += clusters) {
                 if (!mbar_wait(&tempty[acc], acc_ph ^ 1u, status, 72)) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TOK);
-                for (int i = 0; i < steps; ++i) {
-                    if (!mbar_wait(&full[s], ph, status, 73) || !mbar_wait(&a_full[ab], ab_ph, status, 74)) {
+                for (int i = step0; i < step0 + steps; ++i) {
+                    // The decoders have seen `full` (packets and X) before they fill a left factor; X is waited for
+                    // here as well, as its reader is this thread's MMA.
+                    if (!mbar_wait(&a_full[s], ph, status, 74) || !mbar_wait(&full[s], ph, status, 73)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(ab * 32);
+                    const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(s * kTmemStep);
                     const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
+                    const int here = min(kDepth, chunks - i * kDepth);
+                    for (int c = 0; c < here; ++c)
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc_mma_f16_ts(d, a + 8 * kk, xd + 2 * kk, idesc, (i | kk) != 0 ? 1u : 0u);
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma_f16_ts(d, a + 32 * c + 8 * kk, xd + c * (L::x_chunk >> 4) + 2 * kk, idesc,
+                                          (i - step0) | c | kk ? 1u : 0u);
                     tc_commit(&empty[s]);
-                    tc_commit(&a_empty[ab]);
                     if (++s == kStages) {
                         s = 0;
                         ph ^= 1u;
-                    }
-                    if (++ab == kABuffers) {
-                        ab = 0;
-                        ab_ph ^= 1u;
                     }
                 }
                 if (!ok) break;
@@ -415,37 +434,38 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
         }
         __syncwarp();
     } else if (warp >= 6) {
-        // Step q of the CTA (over all its units) goes to set q % kSets, buffer q % kABuffers.
+        // Step q of the CTA (over all its units) goes to set q % kSets, stage q % kStages.
         const int set = (warp - 6) >> 2;
         const int quarter = warp & 3;  // the TMEM lanes a warp may store to
         const int r = quarter * 32 + lane;
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemA;
-        int s = set % kStages, ab = set;  // stage and buffer of this set's next step
-        uint32_t ph = 0, ab_ph = 0;
+        int s = set % kStages;  // stage of this set's next step (kStages >= kSets)
+        uint32_t ph = 0;
         const int my_units = units > cluster ? (units - cluster + clusters - 1) / clusters : 0;
         const int total = my_units * steps;
+        int i = set % steps;  // its place among its unit's steps
         for (int q = set; q < total; q += kSets) {
+            // A full stage is a free one: its loads waited for the last MMAs on its tensor memory too.
             if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, status, 77))) break;
-            const uint8_t* raw = sraw + s * L::raw_bytes;
-            uint32_t w[32];
-            decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, w);
-            if (!__all_sync(0xffffffffu, mbar_wait(&a_empty[ab], ab_ph ^ 1u, status, 78))) break;
             tc_fence_after();
-            tc_st_32x32b_x32(lanes + static_cast<uint32_t>(ab * 32), w);
+            const int here = min(kDepth, chunks - (step0 + i) * kDepth);
+            for (int c = 0; c < here; ++c) {
+                const uint8_t* raw = sraw + s * L::raw_bytes + c * L::packet;
+                uint32_t w[32];
+                decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, w);
+                tc_st_32x32b_x32(lanes + static_cast<uint32_t>(s * kTmemStep + 32 * c), w);
+            }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[ab]);
+            if (lane == 0) mbar_arrive(&a_full[s]);
             s += kSets;
             if (s >= kStages) {
                 s -= kStages;
                 ph ^= 1u;
             }
-            ab += kSets;
-            if (ab >= kABuffers) {
-                ab -= kABuffers;
-                ab_ph ^= 1u;
-            }
+            i += kSets;
+            while (i >= steps) i -= steps;
         }
     } else {
         const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
@@ -586,12 +606,12 @@ void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStre
                         "cudaFuncSetAttribute(routed rows smem)");
     const int tiles = (p.n + 127) / 128 + (p.n % 128 ? 1 : 0);  // of a group, at most
     const int64_t units = std::min<int64_t>(p.rows, p.groups + p.rows / TOK) * tiles;  // at most
-    const int chunks = (p.k + 63) / 64;
+    const int steps = ((p.k + 63) / 64 + kDepth - 1) / kDepth;
     const void* fn = reinterpret_cast<const void*>(kernel);
-    // Few units: the widest cluster that still has every unit resident and leaves a CTA two steps or more.
+    // Few units: the widest cluster that still has every unit resident.
     int split = 1;
-    for (int wide = 2; wide <= kMaxSplit && chunks >= 2 * wide; wide *= 2) {
-        const bool all_work = (wide - 1) * ((chunks + wide - 1) / wide) < chunks;  // no rank without steps
+    for (int wide = 2; wide <= kMaxSplit && steps >= wide; wide *= 2) {
+        const bool all_work = (wide - 1) * ((steps + wide - 1) / wide) < steps;  // no rank without steps
         if (all_work && units <= resident_clusters(state, fn, wide, L::total)) split = wide;
     }
     const int64_t clusters = std::min<int64_t>(units, split > 1 ? resident_clusters(state, fn, split, L::total) : state.sm_count);

@@ -216,13 +216,14 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         const int no_row = static_cast<int>(p.rows);  // an index that reads zeros
         const uint32_t full_bar = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);  // the even CTA's
         const int b_half = rank * (BN / CTAS);
-        // Lane 0: waits for the next stage; the X warp announces the step.
+        // The whole warp waits for the next stage; one thread of the X warp announces the step.
         auto open = [&](bool last) -> bool {
-            if (!mbar_wait(&empty[s], ph ^ 1u, status, 61)) return false;
-            if (is_x && rank == 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 61))) return false;
+            if (is_x && rank == 0 && elect_one()) {
                 last_step[s] = last;
                 mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
             }
+            __syncwarp();
             issued |= 1u << s;
             issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
             return true;
@@ -251,21 +252,21 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 }
                 next = __reduce_min_sync(0xffffffffu, next);
             }
-            if (lane == 0) {
-                const int wrow = t.group * p.n + t.col0 + b_half;
-                const bool plain = next >= p.adapter_count;
-                for (int kb = 0; kb < kblocks; ++kb) {
-                    ok = open(kb == kblocks - 1 && plain);
-                    if (!ok) break;
+            const int wrow = t.group * p.n + t.col0 + b_half;
+            const bool plain = next >= p.adapter_count;
+            for (int kb = 0; kb < kblocks; ++kb) {
+                ok = open(kb == kblocks - 1 && plain);
+                if (!ok) break;
+                if (elect_one()) {
                     if (is_x)
                         tma_tile<CTAS>(sa + s * L::a_bytes, &maps.x, &full[s], full_bar + 8 * s, kb * BK, row0);
                     else
                         tma_tile<CTAS>(sb + s * L::b_bytes, &maps.w, &full[s], full_bar + 8 * s, kb * BK, wrow);
-                    advance();
                 }
+                __syncwarp();
+                advance();
             }
             if (!p.ids) continue;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
             while (ok && next < p.adapter_count) {
                 const int a = next;
                 next = p.adapter_count;
@@ -282,20 +283,19 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 all = __all_sync(0xffffffffu, all);  // no row to mask: a plain tile (rows past the end are not stored)
                 const int4 rows4 = make_int4(v[0], v[1], v[2], v[3]);
                 for (int c = 0; c < 2 * p.rank && ok; c += BK) {
-                    if (lane == 0) {
-                        ok = open(c + BK >= 2 * p.rank && next >= p.adapter_count);
-                        if (ok && !is_x)
+                    ok = open(c + BK >= 2 * p.rank && next >= p.adapter_count);
+                    if (!ok) break;
+                    if (is_x && !all) {
+                        tma_gather4<CTAS>(sa + s * L::a_bytes + lane * 512, &maps.h_rows, full_bar + 8 * s, c, rows4);
+                    } else if (elect_one()) {
+                        if (is_x)
+                            tma_tile<CTAS>(sa + s * L::a_bytes, &maps.h, &full[s], full_bar + 8 * s, c, row0);
+                        else
                             tma_tile<CTAS>(sb + s * L::b_bytes, &maps.b, &full[s], full_bar + 8 * s, c,
                                            a * p.n + t.col0 + b_half);
-                        else if (ok && all)
-                            tma_tile<CTAS>(sa + s * L::a_bytes, &maps.h, &full[s], full_bar + 8 * s, c, row0);
                     }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    const int stage = __shfl_sync(0xffffffffu, s, 0);
-                    if (ok && is_x && !all)
-                        tma_gather4<CTAS>(sa + stage * L::a_bytes + lane * 512, &maps.h_rows, full_bar + 8 * stage, c,
-                                          rows4);
-                    if (lane == 0 && ok) advance();
+                    __syncwarp();
+                    advance();
                 }
             }
         }
@@ -312,7 +312,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             constexpr uint32_t idesc = idesc_f16_f32(CTAS * BM, BN);
             // Descriptors of stage 0; a stage or 32 bytes on only moves the address field (16-byte units).
             const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), b_desc = smem_desc_sw128(smem_u32(sb));
