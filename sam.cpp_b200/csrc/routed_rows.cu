@@ -98,11 +98,18 @@ __device__ __forceinline__ uint32_t half2_of(uint64_t v) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The float whose mantissa holds the bits of `mask` in v: one three-input logic
+// operation (the logic pipe, at half rate, is what bounds the decoders).
+__device__ __forceinline__ float or_into(uint32_t v, uint32_t mask, uint32_t magic) {
+    return __uint_as_float((v & mask) | magic);
+}
+
 // A packet row (codes `code`, scale record `rec`) as f16: word i of `out` holds
-// columns 2 i and 2 i + 1 of the 64.
+// columns 2 i and 2 i + 1 of the 64.  `magic` is 2^23 as bits, in a register: as a
+// second constant beside the mask it would make two operations of or_into.
 template <int TYPE>
 __device__ __forceinline__ void decode_row(const uint8_t* __restrict__ code, const uint8_t* __restrict__ rec,
-                                           uint32_t (&out)[32]) {
+                                           uint32_t magic, uint32_t (&out)[32]) {
     const uint2 record = *reinterpret_cast<const uint2*>(rec);
     if constexpr (TYPE == SAMQ_TYPE_Q8_0) {
         const __half2 bias = __floats2half2_rn(-1152.0f, -1152.0f);  // 1024 of the mantissa trick, 128 of the sign
@@ -133,35 +140,35 @@ __device__ __forceinline__ void decode_row(const uint8_t* __restrict__ code, con
         }
         // Column i of a word's lower (upper, shifted down) half stands at bit 4 (i % 4): worth 16^(i % 4) in the
         // mantissa of 2^23, where up to 23 bits are free.
-        constexpr uint32_t kMagic = 0x4b000000u;
         const float d = __half2float(__ushort_as_half(static_cast<uint16_t>(record.x)));
         if constexpr (TYPE == SAMQ_TYPE_Q6_K) {
             uint32_t high[4];  // 2 bits a column
             *reinterpret_cast<uint4*>(high) = *reinterpret_cast<const uint4*>(code + 32);
+            const uint64_t base = pack2(-8388608.0f, -8388608.0f);
             const uint64_t off01 = pack2(-8388608.0f - 32.0f, -8388608.0f - 512.0f);
             const uint64_t off23 = pack2(-8388608.0f - 8192.0f, -8388608.0f - 131072.0f);
+            // From the bits where they stand (2 i) to 16 times the nibble's unit (4 i + 4).
+            const uint64_t up01 = pack2(16.0f, 64.0f), up23 = pack2(256.0f, 1024.0f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int sc = static_cast<int8_t>((j < 4 ? record.x >> (16 + 8 * (j >> 1)) : record.y >> (8 * ((j >> 1) - 2))) & 0xffu);
                 const float ds = __fmul_rn(d, static_cast<float>(sc));
                 const uint64_t s01 = pack2(ds, ds * 0.0625f), s23 = pack2(ds * 0.00390625f, ds * 0.000244140625f);
-                const uint32_t bits = high[j >> 1] >> (16 * (j & 1));
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const uint32_t n = lo[j] >> (16 * q), b = (bits >> (8 * q)) & 0xffu;
-                    // the two high bits of column i, at bit 4 i + 4
-                    const uint32_t v0 = (n & 0xfu) | ((b << 4) & 0x30u) | kMagic;
-                    const uint32_t v1 = (n & 0xf0u) | ((b << 6) & 0x300u) | kMagic;
-                    const uint32_t v2 = (n & 0xf00u) | ((b << 8) & 0x3000u) | kMagic;
-                    const uint32_t v3 = (n & 0xf000u) | ((b << 10) & 0x30000u) | kMagic;
-                    out[4 * j + 2 * q] = half2_of(mul2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off01), s01));
-                    out[4 * j + 2 * q + 1] =
-                        half2_of(mul2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off23), s23));
+                    const uint32_t n = lo[j] >> (16 * q), b = high[j >> 1] >> (16 * (j & 1) + 8 * q);
+                    const uint64_t h01 = add2(pack2(or_into(b, 0x3u, magic), or_into(b, 0xcu, magic)), base);
+                    const uint64_t h23 = add2(pack2(or_into(b, 0x30u, magic), or_into(b, 0xc0u, magic)), base);
+                    const uint64_t n01 = pack2(or_into(n, 0xfu, magic), or_into(n, 0xf0u, magic));
+                    const uint64_t n23 = pack2(or_into(n, 0xf00u, magic), or_into(n, 0xf000u, magic));
+                    // whole numbers below 2^24: exact
+                    out[4 * j + 2 * q] = half2_of(mul2(add2(fma2(h01, up01, n01), off01), s01));
+                    out[4 * j + 2 * q + 1] = half2_of(mul2(add2(fma2(h23, up23, n23), off23), s23));
                 }
             }
         } else {
             const float dmin = __half2float(__ushort_as_half(static_cast<uint16_t>(record.x >> 16)));
-            const uint64_t off = pack2(-8388608.0f, -8388608.0f);
+            const uint64_t base = pack2(-8388608.0f, -8388608.0f);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float ds = __fmul_rn(d, static_cast<float>((record.y >> (8 * h)) & 0xffu));
@@ -175,20 +182,19 @@ __device__ __forceinline__ void decode_row(const uint8_t* __restrict__ code, con
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const uint32_t n = lo[4 * h + j] >> (16 * q);
-                        uint32_t v0 = (n & 0xfu) | kMagic, v1 = (n & 0xf0u) | kMagic;
-                        uint32_t v2 = (n & 0xf00u) | kMagic, v3 = (n & 0xf000u) | kMagic;
+                        uint64_t v01 = add2(pack2(or_into(n, 0xfu, magic), or_into(n, 0xf0u, magic)), base);
+                        uint64_t v23 = add2(pack2(or_into(n, 0xf00u, magic), or_into(n, 0xf000u, magic)), base);
                         if constexpr (TYPE == SAMQ_TYPE_Q5_K) {
+                            // The fifth bits where they stand (i) to 16 times the nibble's unit (4 i + 4).
                             const uint32_t b = high >> (8 * j + 4 * q);
-                            v0 |= (b << 4) & 0x10u;
-                            v1 |= (b << 7) & 0x100u;
-                            v2 |= (b << 10) & 0x1000u;
-                            v3 |= (b << 13) & 0x10000u;
+                            const uint64_t h01 = add2(pack2(or_into(b, 1u, magic), or_into(b, 2u, magic)), base);
+                            const uint64_t h23 = add2(pack2(or_into(b, 4u, magic), or_into(b, 8u, magic)), base);
+                            v01 = fma2(h01, pack2(16.0f, 128.0f), v01);
+                            v23 = fma2(h23, pack2(1024.0f, 8192.0f), v23);
                         }
                         // ds q has at most 22 bits, so the fused form rounds where the separate one does
-                        out[16 * h + 4 * j + 2 * q] =
-                            half2_of(fma2(add2(pack2(__uint_as_float(v0), __uint_as_float(v1)), off), s01, m2));
-                        out[16 * h + 4 * j + 2 * q + 1] =
-                            half2_of(fma2(add2(pack2(__uint_as_float(v2), __uint_as_float(v3)), off), s23, m2));
+                        out[16 * h + 4 * j + 2 * q] = half2_of(fma2(v01, s01, m2));
+                        out[16 * h + 4 * j + 2 * q + 1] = half2_of(fma2(v23, s23, m2));
                     }
                 }
             }
@@ -441,6 +447,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemA;
         int s = set % kStages;  // stage of this set's next step (kStages >= kSets)
         uint32_t ph = 0;
+        const uint32_t magic = 0x4b000000u + threadIdx.z;  // the compiler does not know that threadIdx.z is 0
         const int my_units = units > cluster ? (units - cluster + clusters - 1) / clusters : 0;
         const int total = my_units * steps;
         int i = set % steps;  // its place among its unit's steps
@@ -452,7 +459,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
             for (int c = 0; c < here; ++c) {
                 const uint8_t* raw = sraw + s * L::raw_bytes + c * L::packet;
                 uint32_t w[32];
-                decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, w);
+                decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, magic, w);
                 tc_st_32x32b_x32(lanes + static_cast<uint32_t>(s * kTmemStep + 32 * c), w);
             }
             tc_wait_st();
