@@ -68,7 +68,7 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
 // groups of either kind and only the device knows which: both kernels run and
 // each leaves the other's groups alone.
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream) {
-    const bool few = p.rows <= kRoutedFewRows;
+    const bool few = p.rows <= (p.ids ? kRoutedFewAdapted : kRoutedFewRows);
     const bool many = !few && (p.groups == 1 || p.rows >= 256 * p.groups);
     if (!many) launch_routed_rows(p, few ? INT_MAX : kRoutedFewRows, state, stream);
     if (!few) launch_routed_tile(p, many ? 1 : kRoutedFewRows + 1, state, stream);

@@ -6,18 +6,22 @@
 // y[i] = act(W_g x[i] + bias_g + delta_i) with the factors swapped: a unit is one
 // packet row tile (128 rows of the stacked weights) of one group by up to TOK of
 // the group's rows, D[128][TOK] = W_tile . X^T in TMEM (tcgen05.mma M = 128,
-// N = TOK).  What bounds it at full size is the packet stream; what bounds it at
+// N = TOK), and for every adapter a that one of the rows names
+// D += [B_a | B_a]_tile . [hi(H) | lo(H)]_a^T with zeros for the rows of others, as
+// in routed_tile.cu.  What bounds it at full size is the packet stream; what bounds it at
 // a few rows is the chain of one unit, so a cluster of SPLIT CTAs shares a unit's
 // depth and adds its partial sums over distributed shared memory, in rank order:
 // one launch, no atomics, no workspace.
 //
 // One CTA per SM, persistent over the units of all groups:
-//   warp 0       each step's packets (kDepth of them, contiguous) by one bulk copy;
-//   last warp    the same columns of X by TMA (rows by index through the row gather);
+//   warp 0       each step's packets (kDepth of them, contiguous) by one bulk copy,
+//                then 128 x 64 of B | B by TMA for each adapter step;
+//   last warp    the same columns of X by TMA (rows by index through the row gather),
+//                hi | lo of the adapter's rows by the row gather;
 //   warp 1       TMEM owner; one thread issues the MMAs;
 //   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
-//                shared memory and back, summed over the cluster), bias, adapters,
-//                erf-GELU, stores coalesced over the weight rows;
+//                shared memory and back, summed over the cluster), bias, erf-GELU,
+//                stores coalesced over the weight rows;
 //   warps 6-     decoders, sets of four on steps in turn: a thread turns a row of its
 //                packets into f16 with the values of packets.cuh bit for bit and stores
 //                it to tensor memory, where the MMA takes it as its left factor.
@@ -51,25 +55,30 @@ constexpr int kTmemStep = 32 * kDepth;  // TMEM columns of a step's left factor:
 constexpr int kMaxGroups = 1024;
 constexpr int kSmemLimit = 232448;
 constexpr int kMaxSplit = 8;
+constexpr int kMaxChunks = kRoutedFewAdapted / 64;  // row chunks of a call with adapters
 
 template <int TYPE, int TOK>
 struct RowsSmem {
     static constexpr int packet = 128 * (code_bytes_of(TYPE) + 8);
     static constexpr int raw_bytes = kDepth * packet;
+    static constexpr int b_bytes = 128 * 128;  // an adapter step's B | B, where the packets lie
+    static constexpr int raw_stage = (raw_bytes > b_bytes ? raw_bytes : b_bytes + 1023) / 1024 * 1024;
     static constexpr int x_chunk = TOK * 128;  // 64 columns of TOK rows
     static constexpr int x_bytes = kDepth * x_chunk;
     static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
     static constexpr int tables = (3 * kMaxGroups + 1) * 4;
-    static constexpr int fixed = 1024 + part + 256 + tables;
+    static constexpr int lists = kMaxChunks * (TOK + 1) * 4;  // the adapters of each row chunk and how many
+    static constexpr int fixed = 1024 + part + 256 + tables + lists;
     // A stage is a step's packets and X in shared memory and its left factor in tensor memory.
-    static constexpr int by_smem = (kSmemLimit - fixed) / (raw_bytes + x_bytes);
+    static constexpr int by_smem = (kSmemLimit - fixed) / (raw_stage + x_bytes);
     static constexpr int by_tmem = (512 - 2 * TOK) / kTmemStep;
     static constexpr int stages = by_smem < by_tmem ? by_smem : by_tmem;
     static constexpr int raw_off = stages * x_bytes;
-    static constexpr int part_off = raw_off + stages * raw_bytes;
+    static constexpr int part_off = raw_off + stages * raw_stage;
     static constexpr int bar_off = part_off + part;
     static constexpr int table_off = bar_off + 256;
-    static constexpr int total = fixed + stages * (raw_bytes + x_bytes);
+    static constexpr int list_off = table_off + tables;
+    static constexpr int total = fixed + stages * (raw_stage + x_bytes);
 };
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -228,6 +237,7 @@ __device__ __forceinline__ int group_tiles(int g, int n) {
 
 struct Unit {
     int group, tile, row0, count;  // packet row tile of the stacked weights, plan rows row0 .. row0 + count - 1
+    int chunk;                     // of the group's rows
 };
 
 template <int TOK>
@@ -243,14 +253,16 @@ __device__ __forceinline__ Unit find_unit(int unit, int n, int groups, const int
     Unit u;
     u.group = lo;
     u.tile = first_tile(lo, n) + at % tiles;
-    u.row0 = s_begin[lo] + at / tiles * TOK;
+    u.chunk = at / tiles;
+    u.row0 = s_begin[lo] + u.chunk * TOK;
     u.count = min(TOK, s_end[lo] - u.row0);
     return u;
 }
 
 template <int TYPE, int TOK>
 __global__ void __launch_bounds__(kThreads, 1)
-routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduct p, int max_rows, int split,
+routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_h,
+                   const __grid_constant__ CUtensorMap map_b, const RoutedProduct p, int max_rows, int split,
                    DeviceStatus* status) {
     using L = RowsSmem<TYPE, TOK>;
     constexpr int kStages = L::stages;
@@ -273,6 +285,8 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
     int* s_end = s_begin + kMaxGroups;
     int* s_first = s_end + kMaxGroups;
+    int* s_count = reinterpret_cast<int*>(smem + L::list_off);  // adapters of each row chunk
+    int* s_list = s_count + kMaxChunks;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
@@ -326,12 +340,41 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
         }
         if (lane == 0) s_first[p.groups] = carry;
     }
+    if (p.ids && warp >= 6 && warp - 6 < kMaxChunks) {
+        // The adapters of row chunk `warp - 6`, in rising order.
+        const int chunk = warp - 6, row0 = chunk * TOK;
+        int id[(TOK + 31) / 32], found = 0, last = -1;
+#pragma unroll
+        for (int j = 0; j < (TOK + 31) / 32; ++j) {
+            const int t = 32 * j + lane;
+            id[j] = t < TOK && row0 + t < p.rows ? __ldg(p.ids + row0 + t) : -1;
+        }
+        for (;;) {
+            int next = p.adapter_count;
+#pragma unroll
+            for (int j = 0; j < (TOK + 31) / 32; ++j)
+                if (id[j] > last) next = min(next, id[j]);
+            next = __reduce_min_sync(0xffffffffu, next);
+            if (next >= p.adapter_count) break;
+            if (lane == 0) s_list[chunk * TOK + found] = next;
+            ++found;
+            last = next;
+        }
+        if (lane == 0) s_count[chunk] = found;
+    }
     tc_fence_before();
     if (split > 1) cluster_sync_all();
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int units = s_first[p.groups];
+    // A unit's steps of this rank: `steps` of packets, then adapter steps rank, rank + split, ... of the
+    // chunk's adapters x the 64-column pieces of their pair.
+    const int pieces = p.ids ? (2 * p.rank + 63) / 64 : 0;
+    auto adapter_steps = [&](int chunk) {
+        const int all = p.ids ? s_count[chunk] * pieces : 0;
+        return all > rank ? (all - rank + split - 1) / split : 0;
+    };
 
     if (warp == 0 || warp == kXWarp) {
         const bool is_x = warp == kXWarp;
@@ -347,25 +390,52 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                 ph ^= 1u;
             }
         };
-        if (is_x && p.row_index) {
+        if (is_x && (p.row_index || p.ids)) {
+            // Rows by index or adapter rows: the whole warp, four rows a lane.
             for (int unit = cluster; unit < units && ok; unit += clusters) {
                 const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
-                int rows[4];
+                int rows[4], id[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * lane + j < u.count ? __ldg(p.row_index + u.row0 + 4 * lane + j) : -1;
+                    const int at = u.row0 + 4 * lane + j;
+                    const bool in = 4 * lane + j < u.count;
+                    const int r = p.row_index && in ? __ldg(p.row_index + at) : -1;
                     rows[j] = r >= 0 && r < p.x_rows ? r : static_cast<int>(p.x_rows);  // past the end: zeros
+                    id[j] = p.ids && in ? __ldg(p.ids + at) : -1;
                 }
                 for (int i = step0; i < step0 + steps; ++i) {
                     const int here = min(kDepth, chunks - i * kDepth);  // packets of this step
                     ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 71));
                     if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                        if (!p.row_index)
+                            for (int c = 0; c < here; ++c)
+                                tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s],
+                                            (i * kDepth + c) * 64, u.row0);
+                    }
                     __syncwarp();
-                    if (lane < TOK / 4)
+                    if (p.row_index && lane < TOK / 4)
                         for (int c = 0; c < here; ++c)
                             gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
                                     (i * kDepth + c) * 64, rows);
+                    advance();
+                }
+                const int more = ok ? adapter_steps(u.chunk) : 0;
+                for (int i = 0; i < more; ++i) {
+                    const int at = rank + i * split;
+                    const int a = s_list[u.chunk * TOK + at / pieces];
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 71));
+                    if (!ok) break;
+                    if (elect_one()) mbar_arrive_expect_tx(&full[s], L::x_chunk);
+                    __syncwarp();
+                    if (lane < TOK / 4) {
+                        int from[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            from[j] = id[j] == a ? u.row0 + 4 * lane + j : static_cast<int>(p.rows);
+                        gather4(sx + s * L::x_bytes + lane * 512, &map_h, &full[s], at % pieces * 64, from);
+                    }
                     advance();
                 }
             }
@@ -379,7 +449,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                     if (!ok) break;
                     if (!is_x) {
                         mbar_arrive_expect_tx(&full[s], here * L::packet);
-                        bulk_load_1d(sraw + s * L::raw_bytes, packet + static_cast<int64_t>(i) * L::raw_bytes,
+                        bulk_load_1d(sraw + s * L::raw_stage, packet + static_cast<int64_t>(i) * L::raw_bytes,
                                      here * L::packet, &full[s]);
                     } else {
                         mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
@@ -387,6 +457,16 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                             tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s], (i * kDepth + c) * 64,
                                         u.row0);
                     }
+                    advance();
+                }
+                const int more = ok ? adapter_steps(u.chunk) : 0;  // none in the X warp's case here
+                for (int i = 0; i < more; ++i) {
+                    const int at = rank + i * split;
+                    const int a = s_list[u.chunk * TOK + at / pieces];
+                    ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&full[s], L::b_bytes);
+                    tma_load_2d(sraw + s * L::raw_stage, &map_b, &full[s], at % pieces * 64, a * p.n + u.tile * 128);
                     advance();
                 }
             }
@@ -400,9 +480,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
     } else if (warp == 1) {
         if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16_f32(128, TOK);
-            const uint64_t x_desc = smem_desc_sw128(smem_u32(sx));
+            const uint64_t x_desc = smem_desc_sw128(smem_u32(sx)), b_desc = smem_desc_sw128(smem_u32(sraw));
             int s = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 0;
+            uint32_t a_phase = 0;  // a stage's left factor is not filled in adapter steps: a phase of its own each
             bool ok = true;
             for (int unit = cluster; unit < units && ok; unit += clusters) {
                 if (!mbar_wait(&tempty[acc], acc_ph ^ 1u, status, 72)) break;
@@ -411,10 +492,11 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                 for (int i = step0; i < step0 + steps; ++i) {
                     // The decoders have seen `full` (packets and X) before they fill a left factor; X is waited for
                     // here as well, as its reader is this thread's MMA.
-                    if (!mbar_wait(&a_full[s], ph, status, 74) || !mbar_wait(&full[s], ph, status, 73)) {
+                    if (!mbar_wait(&a_full[s], a_phase >> s & 1u, status, 74) || !mbar_wait(&full[s], ph, status, 73)) {
                         ok = false;
                         break;
                     }
+                    a_phase ^= 1u << s;
                     tc_fence_after();
                     const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(s * kTmemStep);
                     const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
@@ -424,6 +506,24 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
                         for (int kk = 0; kk < 4; ++kk)
                             tc_mma_f16_ts(d, a + 32 * c + 8 * kk, xd + c * (L::x_chunk >> 4) + 2 * kk, idesc,
                                           (i - step0) | c | kk ? 1u : 0u);
+                    tc_commit(&empty[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                const int more = ok && p.ids ? adapter_steps(find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end).chunk)
+                                             : 0;
+                for (int i = 0; i < more; ++i) {
+                    if (!mbar_wait(&full[s], ph, status, 73)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t bd = b_desc + static_cast<uint32_t>(s * (L::raw_stage >> 4));
+                    const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) tc_mma_f16(d, bd + 2 * kk, xd + 2 * kk, idesc, 1u);
                     tc_commit(&empty[s]);
                     if (++s == kStages) {
                         s = 0;
@@ -440,39 +540,40 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
         }
         __syncwarp();
     } else if (warp >= 6) {
-        // Step q of the CTA (over all its units) goes to set q % kSets, stage q % kStages.
+        // The CTA's packet steps go to the sets in turn; adapter steps pass them by.
         const int set = (warp - 6) >> 2;
         const int quarter = warp & 3;  // the TMEM lanes a warp may store to
         const int r = quarter * 32 + lane;
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemA;
-        int s = set % kStages;  // stage of this set's next step (kStages >= kSets)
-        uint32_t ph = 0;
         const uint32_t magic = 0x4b000000u + threadIdx.z;  // the compiler does not know that threadIdx.z is 0
-        const int my_units = units > cluster ? (units - cluster + clusters - 1) / clusters : 0;
-        const int total = my_units * steps;
-        int i = set % steps;  // its place among its unit's steps
-        for (int q = set; q < total; q += kSets) {
-            // A full stage is a free one: its loads waited for the last MMAs on its tensor memory too.
-            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, status, 77))) break;
-            tc_fence_after();
-            const int here = min(kDepth, chunks - (step0 + i) * kDepth);
-            for (int c = 0; c < here; ++c) {
-                const uint8_t* raw = sraw + s * L::raw_bytes + c * L::packet;
-                uint32_t w[32];
-                decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, magic, w);
-                tc_st_32x32b_x32(lanes + static_cast<uint32_t>(s * kTmemStep + 32 * c), w);
+        int turn = 0;          // the set of the next packet step
+        int before = 0;        // steps of either kind before this unit
+        bool ok = true;
+        for (int unit = cluster; unit < units && ok; unit += clusters) {
+            int i = set - turn;
+            if (i < 0) i += kSets;  // this set's first packet step of the unit
+            for (; i < steps; i += kSets) {
+                const int at = before + i;
+                const int s = at % kStages;
+                // A full stage is a free one: its loads waited for the last MMAs on its tensor memory too.
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], static_cast<uint32_t>(at / kStages) & 1u, status, 77));
+                if (!ok) break;
+                tc_fence_after();
+                const int here = min(kDepth, chunks - (step0 + i) * kDepth);
+                for (int c = 0; c < here; ++c) {
+                    const uint8_t* raw = sraw + s * L::raw_stage + c * L::packet;
+                    uint32_t w[32];
+                    decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, magic, w);
+                    tc_st_32x32b_x32(lanes + static_cast<uint32_t>(s * kTmemStep + 32 * c), w);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[s]);
             }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[s]);
-            s += kSets;
-            if (s >= kStages) {
-                s -= kStages;
-                ph ^= 1u;
-            }
-            i += kSets;
-            while (i >= steps) i -= steps;
+            turn = (turn + steps) % kSets;
+            before += steps;
+            if (p.ids) before += adapter_steps(find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end).chunk);
         }
     } else {
         const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
@@ -490,29 +591,6 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const RoutedProduc
             auto finish = [&](int t, float v) {
                 const int64_t row = u.row0 + t;
                 v += bias;
-                if (p.ids) {
-                    const int a = __ldg(p.ids + row);
-                    if (a >= 0 && a < p.adapter_count && in) {
-                        const uint4* b = reinterpret_cast<const uint4*>(p.b2 + (static_cast<int64_t>(a) * p.n + col) * 2 * p.rank);
-                        const uint4* hp = reinterpret_cast<const uint4*>(p.h2 + row * 2 * p.rank);
-                        const int words = p.rank / 8;
-                        float delta = 0.0f;
-#pragma unroll 2
-                        for (int j = 0; j < words; ++j) {
-                            const uint4 bv = __ldg(b + j), hv = __ldg(hp + j), lv = __ldg(hp + words + j);
-                            const __half2* b2 = reinterpret_cast<const __half2*>(&bv);
-                            const __half2* h2 = reinterpret_cast<const __half2*>(&hv);
-                            const __half2* l2 = reinterpret_cast<const __half2*>(&lv);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 x = __half22float2(b2[i]), y = __half22float2(h2[i]), z = __half22float2(l2[i]);
-                                delta = fmaf(y.x + z.x, x.x, delta);
-                                delta = fmaf(y.y + z.y, x.y, delta);
-                            }
-                        }
-                        v += delta;
-                    }
-                }
                 if (p.gelu) v = gelu_erf(v);
                 if (!in) return;
                 if (f16) static_cast<__half*>(p.y)[row * p.ldy + col] = __float2half_rn(v);
@@ -608,6 +686,14 @@ void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStre
     CUtensorMap map;
     encode_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, p.k, p.x_rows, p.ldx * 2, 64,
                          p.row_index ? 1 : TOK, CU_TENSOR_MAP_SWIZZLE_128B);
+    CUtensorMap map_h = map, map_b = map;
+    if (p.ids) {
+        encode_tensor_map_2d(&map_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, 64, 1,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+        encode_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.b2, 2 * p.rank,
+                             static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank, 64, 128,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+    }
     auto kernel = routed_rows_kernel<TYPE, TOK>;
     set_smem_limit_once(state, reinterpret_cast<const void*>(kernel), L::total,
                         "cudaFuncSetAttribute(routed rows smem)");
@@ -636,7 +722,7 @@ void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStre
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    check_cuda(cudaLaunchKernelEx(&cfg, kernel, map, p, max_rows, split, state.status), "routed_rows_kernel launch");
+    check_cuda(cudaLaunchKernelEx(&cfg, kernel, map, map_h, map_b, p, max_rows, split, state.status), "routed_rows_kernel launch");
 }
 
 template <int TYPE>

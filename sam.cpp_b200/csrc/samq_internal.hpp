@@ -452,7 +452,8 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
                          cudaStream_t stream);
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
-constexpr int kRoutedFewRows = 64;  // rows of a group, at most, that take the packet-streaming kernel
+constexpr int kRoutedFewRows = 64;      // rows of a group, at most, that take the packet-streaming kernel
+constexpr int kRoutedFewAdapted = 256;  // the same for a call with adapters
 // routed_rows.cu: the groups of at most `max_rows` rows from their packets.
 void launch_routed_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream);
 // routed_tile.cu: the groups of at least `min_rows` rows on tensor-core tiles.

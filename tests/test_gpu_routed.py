@@ -416,7 +416,9 @@ def adapters_case(samq, oracle, qtype, k, n, m, max_rank, count, x_dtype, y_dtyp
     (Q8_0, 128, 64, 40, 16, 6, H, F, False, {"ranks": [0, 16, 5, 0, 1, 9]}),
     (Q8_0, 128, 136, 400, 48, 6, H, F, False, {"ranks": [0, 48, 5, 0, 1, 33]}),
     (Q8_0, 64, 40, 9, 4, 2, H, F, False, {"ids": [-1, 2, 1, -(1 << 31), 0, 1 << 30, 1, 0, -7]}),
-    (Q8_0, 64, 40, 200, 4, 2, H, F, False, {"ids": [-1] * 200})])
+    (Q8_0, 64, 40, 200, 4, 2, H, F, False, {"ids": [-1] * 200}),
+    (Q4_K, 2048, 264, 256, 40, 80, H, F, False, {}),
+    (Q8_0, 1024, 1032, 31, 100, 31, F, H, True, {"ids": list(range(31))})])
 def test_adapters(samq, oracle, qtype, k, n, m, rank, count, x_dtype, y_dtype, gelu, extra):
     got, ref, tol = adapters_case(samq, oracle, qtype, k, n, m, rank, count, x_dtype, y_dtype, gelu, **extra)
     assert_close(got, ref, tol)
