@@ -219,10 +219,14 @@ __device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, uint6
         : "memory");
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+// A shared::cta address as that of CTA `rank` of the cluster, and a store there.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    return remote;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ int clamp_row(int v, int64_t rows) {
@@ -240,20 +244,25 @@ struct Unit {
     int chunk;                     // of the group's rows
 };
 
+// Warp-collective: the last group whose first unit is at most `unit`, by two
+// ballots (every 32nd group, then the 32 behind it).
 template <int TOK>
 __device__ __forceinline__ Unit find_unit(int unit, int n, int groups, const int* s_first, const int* s_begin,
-                                          const int* s_end) {
-    int lo = 0, hi = groups;  // s_first[lo] <= unit < s_first[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_first[mid] <= unit) lo = mid;
-        else hi = mid;
+                                          const int* s_end, int lane) {
+    int lo = 0;
+    if (groups > 1) {
+        if (groups > 32) {
+            const bool below = 32 * lane < groups && s_first[32 * lane] <= unit;
+            lo = 32 * (__popc(__ballot_sync(0xffffffffu, below)) - 1);
+        }
+        const bool below = lo + lane < groups && s_first[lo + lane] <= unit;
+        lo += __popc(__ballot_sync(0xffffffffu, below)) - 1;
     }
     const int tiles = group_tiles(lo, n), at = unit - s_first[lo];
     Unit u;
     u.group = lo;
-    u.tile = first_tile(lo, n) + at % tiles;
     u.chunk = at / tiles;
+    u.tile = first_tile(lo, n) + at - u.chunk * tiles;
     u.row0 = s_begin[lo] + u.chunk * TOK;
     u.count = min(TOK, s_end[lo] - u.row0);
     return u;
@@ -277,8 +286,8 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* a_full = empty + kStages;
     uint64_t* tfull = a_full + kStages;
     uint64_t* tempty = tfull + 2;
-    uint64_t* part_full = tempty + 2;   // every CTA of the cluster has written its partial sums
-    uint64_t* part_free = part_full + 1;  // every CTA has read this one's
+    uint64_t* part_full = tempty + 2;     // every CTA of the cluster has sent its partial sums here
+    uint64_t* part_free = part_full + 1;  // every CTA has added up what it was sent
     uint64_t* drain = part_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     static_assert((3 * kStages + 4 + 3) * 8 + 4 <= 256, "barrier space");
@@ -315,8 +324,11 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         tma_prefetch_desc(&map_x);
     }
     if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
-    // What the previous kernel may write is read from here on.
-    pdl_wait();
+    // What the previous kernel may write is read from here on.  With adapters that
+    // kernel is the down product, which began its own work only after everything
+    // before it had completed: all but its pairs may be read at once, and the X
+    // producer waits for those.
+    if (!p.ids) pdl_wait();
     if (warp == 2) {
         int carry = 0;
         for (int base = 0; base < p.groups; base += 32) {
@@ -378,103 +390,103 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
     if (warp == 0 || warp == kXWarp) {
         const bool is_x = warp == kXWarp;
-        int s = 0;
-        uint32_t ph = 0;
-        uint32_t issued = 0, issued_phase = 0;
+        int before = 0;  // steps of either kind before this unit: step i uses stage (before + i) % kStages
         bool ok = true;
-        auto advance = [&] {
-            issued |= 1u << s;
-            issued_phase = (issued_phase & ~(1u << s)) | (ph << s);
-            if (++s == kStages) {
-                s = 0;
-                ph ^= 1u;
-            }
+        auto stage_of = [](int at) { return at % kStages; };
+        auto free_stage = [&](int at) {
+            return mbar_wait(&empty[at % kStages], (static_cast<uint32_t>(at / kStages) & 1u) ^ 1u, status, 71);
         };
-        if (is_x && (p.row_index || p.ids)) {
-            // Rows by index or adapter rows: the whole warp, four rows a lane.
-            for (int unit = cluster; unit < units && ok; unit += clusters) {
-                const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
-                int rows[4], id[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = u.row0 + 4 * lane + j;
-                    const bool in = 4 * lane + j < u.count;
-                    const int r = p.row_index && in ? __ldg(p.row_index + at) : -1;
-                    rows[j] = r >= 0 && r < p.x_rows ? r : static_cast<int>(p.x_rows);  // past the end: zeros
-                    id[j] = p.ids && in ? __ldg(p.ids + at) : -1;
-                }
-                for (int i = step0; i < step0 + steps; ++i) {
-                    const int here = min(kDepth, chunks - i * kDepth);  // packets of this step
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 71));
-                    if (!ok) break;
-                    if (elect_one()) {
-                        mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
-                        if (!p.row_index)
-                            for (int c = 0; c < here; ++c)
-                                tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s],
-                                            (i * kDepth + c) * 64, u.row0);
-                    }
-                    __syncwarp();
-                    if (p.row_index && lane < TOK / 4)
-                        for (int c = 0; c < here; ++c)
-                            gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
-                                    (i * kDepth + c) * 64, rows);
-                    advance();
-                }
-                const int more = ok ? adapter_steps(u.chunk) : 0;
-                for (int i = 0; i < more; ++i) {
-                    const int at = rank + i * split;
-                    const int a = s_list[u.chunk * TOK + at / pieces];
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 71));
-                    if (!ok) break;
-                    if (elect_one()) mbar_arrive_expect_tx(&full[s], L::x_chunk);
-                    __syncwarp();
-                    if (lane < TOK / 4) {
-                        int from[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            from[j] = id[j] == a ? u.row0 + 4 * lane + j : static_cast<int>(p.rows);
-                        gather4(sx + s * L::x_bytes + lane * 512, &map_h, &full[s], at % pieces * 64, from);
-                    }
-                    advance();
-                }
-            }
-        } else if (elect_one()) {
-            for (int unit = cluster; unit < units && ok; unit += clusters) {
-                const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
-                const uint8_t* packet = p.packets + static_cast<int64_t>(u.tile) * chunks * L::packet;
-                for (int i = step0; i < step0 + steps; ++i) {
-                    const int here = min(kDepth, chunks - i * kDepth);
-                    ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
-                    if (!ok) break;
-                    if (!is_x) {
+        for (int unit = cluster; unit < units && ok; unit += clusters) {
+            const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end, lane);
+            const int more = adapter_steps(u.chunk);
+            if (!is_x) {
+                // One thread issues the unit's packets and adapter tiles.
+                if (elect_one()) {
+                    const uint8_t* packet = p.packets + static_cast<int64_t>(u.tile) * chunks * L::packet;
+                    for (int i = 0; i < steps; ++i) {
+                        const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
+                        if (!(ok = free_stage(before + i))) break;
+                        const int s = stage_of(before + i);
                         mbar_arrive_expect_tx(&full[s], here * L::packet);
-                        bulk_load_1d(sraw + s * L::raw_stage, packet + static_cast<int64_t>(i) * L::raw_bytes,
+                        bulk_load_1d(sraw + s * L::raw_stage, packet + static_cast<int64_t>(c0) * L::packet,
                                      here * L::packet, &full[s]);
-                    } else {
-                        mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
-                        for (int c = 0; c < here; ++c)
-                            tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s], (i * kDepth + c) * 64,
-                                        u.row0);
                     }
-                    advance();
+                    for (int i = 0; i < more && ok; ++i) {
+                        if (!(ok = free_stage(before + steps + i))) break;
+                        const int s = stage_of(before + steps + i), at = rank + i * split;
+                        const int a = s_list[u.chunk * TOK + at / pieces];
+                        mbar_arrive_expect_tx(&full[s], L::b_bytes);
+                        tma_load_2d(sraw + s * L::raw_stage, &map_b, &full[s], at % pieces * 64,
+                                    a * p.n + u.tile * 128);
+                    }
                 }
-                const int more = ok ? adapter_steps(u.chunk) : 0;  // none in the X warp's case here
-                for (int i = 0; i < more; ++i) {
-                    const int at = rank + i * split;
-                    const int a = s_list[u.chunk * TOK + at / pieces];
-                    ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
-                    if (!ok) break;
-                    mbar_arrive_expect_tx(&full[s], L::b_bytes);
-                    tma_load_2d(sraw + s * L::raw_stage, &map_b, &full[s], at % pieces * 64, a * p.n + u.tile * 128);
-                    advance();
+                __syncwarp();
+            } else {
+                if (!p.row_index) {
+                    if (elect_one())
+                        for (int i = 0; i < steps; ++i) {
+                            const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
+                            if (!(ok = free_stage(before + i))) break;
+                            const int s = stage_of(before + i);
+                            mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                            for (int c = 0; c < here; ++c)
+                                tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s], (c0 + c) * 64,
+                                            u.row0);
+                        }
+                    __syncwarp();
+                }
+                // Rows by index and adapter rows: four rows a lane.
+                const int first = p.row_index ? 0 : steps;
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok && first < steps + more) {
+                    int rows[4], id[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = u.row0 + 4 * lane + j;
+                        const bool in = 4 * lane + j < u.count;
+                        const int r = p.row_index && in ? __ldg(p.row_index + at) : -1;
+                        rows[j] = r >= 0 && r < p.x_rows ? r : static_cast<int>(p.x_rows);  // past the end: zeros
+                        id[j] = p.ids && in ? __ldg(p.ids + at) : -1;
+                    }
+                    if (more) pdl_wait();  // the pairs of the down product
+                    for (int i = first; i < steps + more; ++i) {
+                        const int s = stage_of(before + i);
+                        if (elect_one()) ok = free_stage(before + i);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (i < steps) {
+                            const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
+                            if (elect_one()) mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                            __syncwarp();
+                            if (lane < TOK / 4)
+                                for (int c = 0; c < here; ++c)
+                                    gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
+                                            (c0 + c) * 64, rows);
+                        } else {
+                            const int at = rank + (i - steps) * split;
+                            const int a = s_list[u.chunk * TOK + at / pieces];
+                            if (elect_one()) mbar_arrive_expect_tx(&full[s], L::x_chunk);
+                            __syncwarp();
+                            if (lane < TOK / 4) {
+                                int from[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    from[j] = id[j] == a ? u.row0 + 4 * lane + j : static_cast<int>(p.rows);
+                                gather4(sx + s * L::x_bytes + lane * 512, &map_h, &full[s], at % pieces * 64, from);
+                            }
+                        }
+                    }
                 }
             }
+            ok = __all_sync(0xffffffffu, ok);
+            before += steps + more;
         }
-        pdl_trigger();  // this thread's loads are issued
-        if (!ok) {  // let the copies in flight land before the CTA exits
-            for (int i = 0; i < kStages; ++i)
-                if (issued & (1u << i)) mbar_wait(&full[i], (issued_phase >> i) & 1u, status, 75);
+        if (is_x) pdl_wait();  // if not before: the kernel ends after its predecessors
+        pdl_trigger();  // this warp's loads are issued
+        if (!ok && lane == 0) {
+            // A wait gave up: time for the copies in flight to land before the CTA exits.
+            const uint64_t start = global_timer_ns();
+            while (global_timer_ns() - start < 2000000ull) __nanosleep(1000);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -512,8 +524,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                         ph ^= 1u;
                     }
                 }
-                const int more = ok && p.ids ? adapter_steps(find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end).chunk)
-                                             : 0;
+                const int more = ok && p.ids ? adapter_steps(unit / group_tiles(0, p.n)) : 0;
                 for (int i = 0; i < more; ++i) {
                     if (!mbar_wait(&full[s], ph, status, 73)) {
                         ok = false;
@@ -573,28 +584,42 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             }
             turn = (turn + steps) % kSets;
             before += steps;
-            if (p.ids) before += adapter_steps(find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end).chunk);
+            if (p.ids) before += adapter_steps(unit / group_tiles(0, p.n));  // one group
         }
     } else {
         const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
         const int mine = quarter * 32 + lane;
         const bool f16 = p.y_type == SAMQ_TYPE_F16;
+        const int shift = 31 - __clz(split);  // split is a power of two
+        const int share = TOK >> shift;       // rows that a CTA of the cluster finishes: t % split == rank
         int acc = 0;
         uint32_t acc_ph = 0, part_ph = 0;
+        // The next unit's place and bias are fetched under this one's wait.
+        Unit u{}, next{};
+        float bias = 0.0f, next_bias = 0.0f;
+        auto fetch = [&](int unit) {
+            if (unit >= units) return;
+            next = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end, lane);
+            const int64_t col = static_cast<int64_t>(next.tile) * 128 + mine - static_cast<int64_t>(next.group) * p.n;
+            next_bias = p.bias && col >= 0 && col < p.n ? __ldg(p.bias + static_cast<int64_t>(next.group) * p.n + col)
+                                                        : 0.0f;
+        };
+        fetch(cluster);
         for (int unit = cluster; unit < units; unit += clusters) {
-            const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end);
+            u = next;
+            bias = next_bias;
+            fetch(unit + clusters);
             // This lane's weight row as a column of the group's output.
-            const int64_t col64 = static_cast<int64_t>(u.tile) * 128 + mine - static_cast<int64_t>(u.group) * p.n;
-            const bool in = col64 >= 0 && col64 < p.n;
-            const int col = static_cast<int>(col64);
-            const float bias = in && p.bias ? __ldg(p.bias + static_cast<int64_t>(u.group) * p.n + col) : 0.0f;
+            const int64_t col = static_cast<int64_t>(u.tile) * 128 + mine - static_cast<int64_t>(u.group) * p.n;
+            const bool in = col >= 0 && col < p.n;
+            const int64_t at0 = u.row0 * p.ldy + col;
             auto finish = [&](int t, float v) {
-                const int64_t row = u.row0 + t;
                 v += bias;
                 if (p.gelu) v = gelu_erf(v);
                 if (!in) return;
-                if (f16) static_cast<__half*>(p.y)[row * p.ldy + col] = __float2half_rn(v);
-                else static_cast<float*>(p.y)[row * p.ldy + col] = v;
+                const int64_t at = at0 + t * p.ldy;
+                if (f16) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
+                else static_cast<float*>(p.y)[at] = v;
             };
             // Warp-uniform: the TMEM loads below are warp-collective.
             if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 79))) break;
@@ -611,8 +636,14 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 else tc_ld_32x32b_x32(d + c, v);
                 tc_wait_ld();
                 if (split > 1) {
+                    // Row t to CTA t % split: slot [this rank][t / split] of its partial sums.
+                    const uint32_t slot = smem_u32(spart + rank * share * 128 + mine);
 #pragma unroll
-                    for (int i = 0; i < C; ++i) spart[(c + i) * 128 + mine] = __uint_as_float(v[i]);
+                    for (int i = 0; i < C; ++i) {
+                        const int t = c + i;
+                        if (t < u.count)
+                            st_cluster(map_rank(slot + (t >> shift) * 512, t & (split - 1)), __uint_as_float(v[i]));
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < C; ++i)
@@ -628,14 +659,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             if (split > 1) {
                 if (lane < split) mbar_arrive_cluster(cluster_map(part_full, lane));
                 if (!__all_sync(0xffffffffu, mbar_wait_cluster(part_full, part_ph, status, 81))) break;
-                const uint32_t own = smem_u32(spart + mine);
                 for (int t = rank; t < u.count; t += split) {
+                    const float* from = spart + (t >> shift) * 128 + mine;
                     float v = 0.0f;
-                    for (int o = 0; o < split; ++o) {
-                        uint32_t remote;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(own + t * 512), "r"(o));
-                        v += ld_cluster(remote);
-                    }
+                    for (int o = 0; o < split; ++o) v += from[o * share * 128];
                     finish(t, v);
                 }
                 __syncwarp();

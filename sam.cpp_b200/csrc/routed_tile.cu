@@ -174,8 +174,11 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         if constexpr (CTAS == 2) tmem_alloc_pair(tmem_slot, 2 * kAccStride);
         else tmem_alloc(tmem_slot, 2 * kAccStride);
     }
-    // What the previous kernel may write is read from here on.
-    pdl_wait();
+    // What the previous kernel may write is read from here on.  With adapters that
+    // kernel is the down product, which began its own work only after everything
+    // before it had completed: all but its pairs may be read at once, and the X
+    // producer waits for those.
+    if (!p.ids) pdl_wait();
     if (warp == 2) {
         int carry = 0;
         for (int base = 0; base < p.groups; base += 32) {
@@ -218,7 +221,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         const int b_half = rank * (BN / CTAS);
         // The whole warp waits for the next stage; one thread of the X warp announces the step.
         auto open = [&](bool last) -> bool {
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, status, 61))) return false;
+            if (!mbar_wait_warp(&empty[s], ph ^ 1u, status, 61)) return false;
             if (is_x && rank == 0 && elect_one()) {
                 last_step[s] = last;
                 mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
@@ -267,6 +270,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 advance();
             }
             if (!p.ids) continue;
+            if (is_x && ok && next < p.adapter_count) pdl_wait();
             while (ok && next < p.adapter_count) {
                 const int a = next;
                 next = p.adapter_count;
@@ -299,7 +303,8 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 }
             }
         }
-        pdl_trigger();  // all of this warp's loads are issued
+        if (is_x) pdl_wait();  // if not before: the kernel ends after its predecessors
+        pdl_trigger();         // all of this warp's loads are issued
         if (!ok && lane == 0) {
             // Let the copies in flight land before the CTA exits.
             if constexpr (CTAS == 1) {
@@ -389,7 +394,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             const float* bias = p.bias ? p.bias + static_cast<int64_t>(t.group) * p.n + t.col0 : nullptr;
             const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15u) == 0;
             // Warp-uniform: the TMEM loads below are warp-collective.
-            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 64))) break;
+            if (!mbar_wait_warp(&tfull[acc], acc_ph, status, 64)) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = part * kShare; c0 < (part + 1) * kShare; c0 += slab_cols) {

@@ -146,6 +146,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, Device
     }
 }
 
+// mbar_wait for a converged warp: one thread waits (32 lanes on one barrier cost
+// 32 probes), the others take its word; all of them may then read what the phase
+// published.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, DeviceStatus* status, uint32_t site) {
+    bool ok = true;
+    if (elect_one()) ok = mbar_wait(bar, parity, status, site);
+    return __all_sync(0xffffffffu, ok);
+}
+
 // ---- Q8_1 activation operand ---------------------------------------------
 // The staging rule of GGML CUDA's quantize_q8_1 as pinned by SAM.cpp's
 // verifiers (tools/validation/verify_q8_rhs_staging.py:24-83) and scale patch
