@@ -14,21 +14,22 @@
 // one launch, no atomics, no workspace.
 //
 // One CTA per SM, persistent over the units of all groups:
-//   warp 0       each step's packets (kDepth of them, contiguous) by one bulk copy,
-//                then 128 x 64 of B | B by TMA for each adapter step;
+//   warp 0       packets, kLoad contiguous ones by one bulk copy, then 128 x 64 of
+//                B | B by TMA for each adapter step;
 //   last warp    the same columns of X by TMA (rows by index through the row gather),
 //                hi | lo of the adapter's rows by the row gather;
 //   warp 1       TMEM owner; one thread issues the MMAs;
 //   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
-//                shared memory and back, summed over the cluster), bias, erf-GELU,
+//                shared memory of the CTA that adds up the row), bias, erf-GELU,
 //                stores coalesced over the weight rows;
-//   warps 6-     decoders, sets of four on steps in turn: a thread turns a row of its
-//                packets into f16 with the values of packets.cuh bit for bit and stores
-//                it to tensor memory, where the MMA takes it as its left factor.
-// A step costs the thread that issues its copies about 250 cycles and the MMA
-// thread as much whatever its size, while a Q4_K packet takes 210 cycles of HBM
-// bandwidth: hence kDepth packets a step, one thread per kind of copy, and one
-// barrier pair for a step's shared and tensor memory.
+//   warps 6-     decoders, sets of four on steps of kDepth packets in turn: a thread
+//                turns a row of its packets into f16 with the values of packets.cuh bit
+//                for bit and stores it to tensor memory, where the MMA takes it as its
+//                left factor.
+// Beside the decoders, who fill the issue slots, a copy costs the thread that
+// issues it about 500 cycles and a step the MMA thread 400, while a Q4_K packet
+// takes 210 cycles of HBM bandwidth: hence several packets a copy and a step, and
+// one thread per kind of copy.
 // The decoders' arithmetic: a nibble becomes a float by or-ing it into the
 // mantissa of 2^23 where it stands (the sub-block's scale takes the power of 16),
 // and pairs of weights share packed f32 operations; an int8 becomes a half by the
@@ -50,7 +51,7 @@ constexpr int kDecodeWarps = 16;
 constexpr int kXWarp = 6 + kDecodeWarps;
 constexpr int kThreads = 32 * (kXWarp + 1);
 constexpr int kSets = kDecodeWarps / 4;
-constexpr int kDepth = 2;             // packets (64 columns each) of a step
+constexpr int kDepth = 2;               // packets (64 columns each) of a step
 constexpr int kTmemStep = 32 * kDepth;  // TMEM columns of a step's left factor: 128 rows x 64 kDepth f16
 constexpr int kMaxGroups = 1024;
 constexpr int kSmemLimit = 232448;
@@ -60,23 +61,23 @@ constexpr int kMaxChunks = kRoutedFewAdapted / 64;  // row chunks of a call with
 template <int TYPE, int TOK>
 struct RowsSmem {
     static constexpr int packet = 128 * (code_bytes_of(TYPE) + 8);
-    static constexpr int raw_bytes = kDepth * packet;
+    static constexpr int load = TOK == 64 ? 2 : 4;  // packets of a copy
+    static constexpr int raw_bytes = load * packet;
     static constexpr int b_bytes = 128 * 128;  // an adapter step's B | B, where the packets lie
     static constexpr int raw_stage = (raw_bytes > b_bytes ? raw_bytes : b_bytes + 1023) / 1024 * 1024;
     static constexpr int x_chunk = TOK * 128;  // 64 columns of TOK rows
-    static constexpr int x_bytes = kDepth * x_chunk;
+    static constexpr int x_bytes = load * x_chunk;
     static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
     static constexpr int tables = (3 * kMaxGroups + 1) * 4;
     static constexpr int lists = kMaxChunks * (TOK + 1) * 4;  // the adapters of each row chunk and how many
-    static constexpr int fixed = 1024 + part + 256 + tables + lists;
-    // A stage is a step's packets and X in shared memory and its left factor in tensor memory.
-    static constexpr int by_smem = (kSmemLimit - fixed) / (raw_stage + x_bytes);
-    static constexpr int by_tmem = (512 - 2 * TOK) / kTmemStep;
-    static constexpr int stages = by_smem < by_tmem ? by_smem : by_tmem;
+    static constexpr int fixed = 1024 + part + 512 + tables + lists;
+    static constexpr int fit = (kSmemLimit - fixed) / (raw_stage + x_bytes);
+    static constexpr int stages = fit > 8 ? 8 : fit;
+    static constexpr int slots = (512 - 2 * TOK) / kTmemStep < 8 ? (512 - 2 * TOK) / kTmemStep : 8;  // left factors
     static constexpr int raw_off = stages * x_bytes;
     static constexpr int part_off = raw_off + stages * raw_stage;
     static constexpr int bar_off = part_off + part;
-    static constexpr int table_off = bar_off + 256;
+    static constexpr int table_off = bar_off + 512;
     static constexpr int list_off = table_off + tables;
     static constexpr int total = fixed + stages * (raw_stage + x_bytes);
 };
@@ -274,8 +275,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                    const __grid_constant__ CUtensorMap map_b, const RoutedProduct p, int max_rows, int split,
                    DeviceStatus* status) {
     using L = RowsSmem<TYPE, TOK>;
-    constexpr int kStages = L::stages;
-    static_assert(kStages >= kSets && L::total <= kSmemLimit, "shared memory budget");
+    constexpr int kStages = L::stages, kSlots = L::slots, kLoad = L::load;
+    constexpr int kSteps = kLoad / kDepth;  // of a copy
+    static_assert(kStages >= 2 && kSlots >= kSets && L::total <= kSmemLimit, "shared memory budget");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sx = smem;
@@ -284,13 +286,14 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off);
     uint64_t* empty = full + kStages;
     uint64_t* a_full = empty + kStages;
-    uint64_t* tfull = a_full + kStages;
+    uint64_t* a_empty = a_full + kSlots;
+    uint64_t* tfull = a_empty + kSlots;
     uint64_t* tempty = tfull + 2;
     uint64_t* part_full = tempty + 2;     // every CTA of the cluster has sent its partial sums here
     uint64_t* part_free = part_full + 1;  // every CTA has added up what it was sent
     uint64_t* drain = part_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    static_assert((3 * kStages + 4 + 3) * 8 + 4 <= 256, "barrier space");
+    static_assert((2 * kStages + 2 * kSlots + 4 + 3) * 8 + 4 <= 512, "barrier space");
     int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
     int* s_end = s_begin + kMaxGroups;
     int* s_first = s_end + kMaxGroups;
@@ -311,7 +314,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 2);
             mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kSlots; ++s) {
             mbar_init(&a_full[s], 4);
+            mbar_init(&a_empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
@@ -380,6 +386,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int units = s_first[p.groups];
+    const int loads = (steps + kSteps - 1) / kSteps;  // copies of a unit's packets
     // A unit's steps of this rank: `steps` of packets, then adapter steps rank, rank + split, ... of the
     // chunk's adapters x the 64-column pieces of their pair.
     const int pieces = p.ids ? (2 * p.rank + 63) / 64 : 0;
@@ -390,55 +397,67 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
     if (warp == 0 || warp == kXWarp) {
         const bool is_x = warp == kXWarp;
-        int before = 0;  // steps of either kind before this unit: step i uses stage (before + i) % kStages
+        int before = 0;  // copies before this unit: copy i uses stage (before + i) % kStages
         bool ok = true;
-        auto stage_of = [](int at) { return at % kStages; };
-        auto free_stage = [&](int at) {
-            return mbar_wait(&empty[at % kStages], (static_cast<uint32_t>(at / kStages) & 1u) ^ 1u, status, 71);
-        };
         for (int unit = cluster; unit < units && ok; unit += clusters) {
             const Unit u = find_unit<TOK>(unit, p.n, p.groups, s_first, s_begin, s_end, lane);
             const int more = adapter_steps(u.chunk);
+            int s = before % kStages;
+            uint32_t ph = static_cast<uint32_t>(before / kStages) & 1u;
+            auto advance = [&] {
+                if (++s == kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            };
             if (!is_x) {
                 // One thread issues the unit's packets and adapter tiles.
                 if (elect_one()) {
-                    const uint8_t* packet = p.packets + static_cast<int64_t>(u.tile) * chunks * L::packet;
-                    for (int i = 0; i < steps; ++i) {
-                        const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
-                        if (!(ok = free_stage(before + i))) break;
-                        const int s = stage_of(before + i);
-                        mbar_arrive_expect_tx(&full[s], here * L::packet);
-                        bulk_load_1d(sraw + s * L::raw_stage, packet + static_cast<int64_t>(c0) * L::packet,
-                                     here * L::packet, &full[s]);
+                    const int left = min(chunks - step0 * kDepth, steps * kDepth);
+                    const uint8_t* from =
+                        p.packets + (static_cast<int64_t>(u.tile) * chunks + step0 * kDepth) * L::packet;
+                    for (int c = 0; c < left; c += kLoad) {
+                        if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
+                        const int bytes = min(kLoad, left - c) * L::packet;
+                        mbar_arrive_expect_tx(&full[s], bytes);
+                        bulk_load_1d(sraw + s * L::raw_stage, from, bytes, &full[s]);
+                        from += L::raw_bytes;
+                        advance();
                     }
                     for (int i = 0; i < more && ok; ++i) {
-                        if (!(ok = free_stage(before + steps + i))) break;
-                        const int s = stage_of(before + steps + i), at = rank + i * split;
+                        if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
+                        const int at = rank + i * split;
                         const int a = s_list[u.chunk * TOK + at / pieces];
                         mbar_arrive_expect_tx(&full[s], L::b_bytes);
                         tma_load_2d(sraw + s * L::raw_stage, &map_b, &full[s], at % pieces * 64,
                                     a * p.n + u.tile * 128);
+                        advance();
                     }
                 }
                 __syncwarp();
             } else {
                 if (!p.row_index) {
                     if (elect_one())
-                        for (int i = 0; i < steps; ++i) {
-                            const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
-                            if (!(ok = free_stage(before + i))) break;
-                            const int s = stage_of(before + i);
-                            mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
-                            for (int c = 0; c < here; ++c)
-                                tma_load_2d(sx + s * L::x_bytes + c * L::x_chunk, &map_x, &full[s], (c0 + c) * 64,
-                                            u.row0);
+                        for (int c = step0 * kDepth; c < min(chunks, (step0 + steps) * kDepth); c += kLoad) {
+                            if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
+                            if (p.k % 64 == 0) {  // one copy; the chunks past the end read zeros
+                                mbar_arrive_expect_tx(&full[s], L::x_bytes);
+                                tma_load_3d(sx + s * L::x_bytes, &map_x, &full[s], 0, u.row0, c);
+                            } else {
+                                const int here = min(kLoad, chunks - c);
+                                mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
+                                for (int j = 0; j < here; ++j)
+                                    tma_load_2d(sx + s * L::x_bytes + j * L::x_chunk, &map_x, &full[s], (c + j) * 64,
+                                                u.row0);
+                            }
+                            advance();
                         }
                     __syncwarp();
                 }
                 // Rows by index and adapter rows: four rows a lane.
-                const int first = p.row_index ? 0 : steps;
+                const int first = p.row_index ? 0 : loads;
                 ok = __all_sync(0xffffffffu, ok);
-                if (ok && first < steps + more) {
+                if (ok && first < loads + more) {
                     int rows[4], id[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -449,13 +468,15 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                         id[j] = p.ids && in ? __ldg(p.ids + at) : -1;
                     }
                     if (more) pdl_wait();  // the pairs of the down product
-                    for (int i = first; i < steps + more; ++i) {
-                        const int s = stage_of(before + i);
-                        if (elect_one()) ok = free_stage(before + i);
+                    s = (before + first) % kStages;
+                    ph = static_cast<uint32_t>((before + first) / kStages) & 1u;
+                    for (int i = first; i < loads + more; ++i) {
+                        if (elect_one()) ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
-                        if (i < steps) {
-                            const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
+                        if (i < loads) {
+                            const int c0 = step0 * kDepth + i * kLoad;
+                            const int here = min(kLoad, min(chunks, (step0 + steps) * kDepth) - c0);
                             if (elect_one()) mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
                             __syncwarp();
                             if (lane < TOK / 4)
@@ -463,7 +484,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                                     gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
                                             (c0 + c) * 64, rows);
                         } else {
-                            const int at = rank + (i - steps) * split;
+                            const int at = rank + (i - loads) * split;
                             const int a = s_list[u.chunk * TOK + at / pieces];
                             if (elect_one()) mbar_arrive_expect_tx(&full[s], L::x_chunk);
                             __syncwarp();
@@ -475,11 +496,12 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                                 gather4(sx + s * L::x_bytes + lane * 512, &map_h, &full[s], at % pieces * 64, from);
                             }
                         }
+                        advance();
                     }
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
-            before += steps + more;
+            before += loads + more;
         }
         if (is_x) pdl_wait();  // if not before: the kernel ends after its predecessors
         pdl_trigger();  // this warp's loads are issued
@@ -493,35 +515,45 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16_f32(128, TOK);
             const uint64_t x_desc = smem_desc_sw128(smem_u32(sx)), b_desc = smem_desc_sw128(smem_u32(sraw));
-            int s = 0, acc = 0;
-            uint32_t ph = 0, acc_ph = 0;
-            uint32_t a_phase = 0;  // a stage's left factor is not filled in adapter steps: a phase of its own each
+            int s = 0, slot = 0, acc = 0;
+            uint32_t ph = 0, slot_ph = 0, acc_ph = 0;
             bool ok = true;
+            auto advance = [&] {
+                if (++s == kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            };
             for (int unit = cluster; unit < units && ok; unit += clusters) {
                 if (!mbar_wait(&tempty[acc], acc_ph ^ 1u, status, 72)) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TOK);
-                for (int i = step0; i < step0 + steps; ++i) {
-                    // The decoders have seen `full` (packets and X) before they fill a left factor; X is waited for
-                    // here as well, as its reader is this thread's MMA.
-                    if (!mbar_wait(&a_full[s], a_phase >> s & 1u, status, 74) || !mbar_wait(&full[s], ph, status, 73)) {
+                for (int i = 0; i < steps; ++i) {
+                    const int part = i % kSteps;  // of its copy
+                    if ((part == 0 && !mbar_wait(&full[s], ph, status, 73)) ||
+                        !mbar_wait(&a_full[slot], slot_ph, status, 74)) {
                         ok = false;
                         break;
                     }
-                    a_phase ^= 1u << s;
                     tc_fence_after();
-                    const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(s * kTmemStep);
-                    const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
-                    const int here = min(kDepth, chunks - i * kDepth);
-                    for (int c = 0; c < here; ++c)
+                    const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(slot * kTmemStep);
+                    const uint64_t xd = x_desc + static_cast<uint32_t>((s * L::x_bytes + part * kDepth * L::x_chunk) >> 4);
+                    const int here = min(kDepth, chunks - (step0 + i) * kDepth);
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc_mma_f16_ts(d, a + 32 * c + 8 * kk, xd + c * (L::x_chunk >> 4) + 2 * kk, idesc,
-                                          (i - step0) | c | kk ? 1u : 0u);
-                    tc_commit(&empty[s]);
-                    if (++s == kStages) {
-                        s = 0;
-                        ph ^= 1u;
+                    for (int c = 0; c < kDepth; ++c)
+                        if (c < here)
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                tc_mma_f16_ts(d, a + 32 * c + 8 * kk, xd + c * (L::x_chunk >> 4) + 2 * kk, idesc,
+                                              i | c | kk ? 1u : 0u);
+                    tc_commit(&a_empty[slot]);
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        slot_ph ^= 1u;
+                    }
+                    if (part == kSteps - 1 || i == steps - 1) {
+                        tc_commit(&empty[s]);
+                        advance();
                     }
                 }
                 const int more = ok && p.ids ? adapter_steps(unit / group_tiles(0, p.n)) : 0;
@@ -536,10 +568,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) tc_mma_f16(d, bd + 2 * kk, xd + 2 * kk, idesc, 1u);
                     tc_commit(&empty[s]);
-                    if (++s == kStages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
+                    advance();
                 }
                 if (!ok) break;
                 tc_commit(&tfull[acc]);
@@ -551,40 +580,41 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         }
         __syncwarp();
     } else if (warp >= 6) {
-        // The CTA's packet steps go to the sets in turn; adapter steps pass them by.
+        // The CTA's packet steps go to the sets and slots in turn.
         const int set = (warp - 6) >> 2;
         const int quarter = warp & 3;  // the TMEM lanes a warp may store to
         const int r = quarter * 32 + lane;
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemA;
         const uint32_t magic = 0x4b000000u + threadIdx.z;  // the compiler does not know that threadIdx.z is 0
-        int turn = 0;          // the set of the next packet step
-        int before = 0;        // steps of either kind before this unit
+        int done = 0;    // packet steps before this unit
+        int copies = 0;  // copies of either kind before this unit
         bool ok = true;
         for (int unit = cluster; unit < units && ok; unit += clusters) {
-            int i = set - turn;
-            if (i < 0) i += kSets;  // this set's first packet step of the unit
+            int i = set - done % kSets;
+            if (i < 0) i += kSets;  // this set's first step of the unit
             for (; i < steps; i += kSets) {
-                const int at = before + i;
-                const int s = at % kStages;
-                // A full stage is a free one: its loads waited for the last MMAs on its tensor memory too.
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], static_cast<uint32_t>(at / kStages) & 1u, status, 77));
+                const int copy = copies + i / kSteps, s = copy % kStages;
+                const int step = done + i, slot = step % kSlots;
+                ok = __all_sync(0xffffffffu,
+                                mbar_wait(&full[s], static_cast<uint32_t>(copy / kStages) & 1u, status, 77) &&
+                                    mbar_wait(&a_empty[slot], (static_cast<uint32_t>(step / kSlots) & 1u) ^ 1u, status, 78));
                 if (!ok) break;
                 tc_fence_after();
                 const int here = min(kDepth, chunks - (step0 + i) * kDepth);
                 for (int c = 0; c < here; ++c) {
-                    const uint8_t* raw = sraw + s * L::raw_stage + c * L::packet;
+                    const uint8_t* raw = sraw + s * L::raw_stage + (i % kSteps * kDepth + c) * L::packet;
                     uint32_t w[32];
                     decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, magic, w);
-                    tc_st_32x32b_x32(lanes + static_cast<uint32_t>(s * kTmemStep + 32 * c), w);
+                    tc_st_32x32b_x32(lanes + static_cast<uint32_t>(slot * kTmemStep + 32 * c), w);
                 }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[s]);
+                if (lane == 0) mbar_arrive(&a_full[slot]);
             }
-            turn = (turn + steps) % kSets;
-            before += steps;
-            if (p.ids) before += adapter_steps(unit / group_tiles(0, p.n));  // one group
+            done += steps;
+            copies += loads;
+            if (p.ids) copies += adapter_steps(unit / group_tiles(0, p.n));  // one group
         }
     } else {
         const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
@@ -711,13 +741,18 @@ template <int TYPE, int TOK>
 void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream) {
     using L = RowsSmem<TYPE, TOK>;
     CUtensorMap map;
-    encode_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, p.k, p.x_rows, p.ldx * 2, 64,
-                         p.row_index ? 1 : TOK, CU_TENSOR_MAP_SWIZZLE_128B);
+    const auto f16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (!p.row_index && p.k % 64 == 0)  // [k / 64][x_rows][64]: several 64-column chunks a copy
+        encode_tensor_map_3d_box(&map, f16, p.x, 64, p.x_rows, p.k / 64, p.ldx * 2, 128, 64, TOK, L::load,
+                                 CU_TENSOR_MAP_SWIZZLE_128B);
+    else
+        encode_tensor_map_2d(&map, f16, p.x, p.k, p.x_rows, p.ldx * 2, 64, p.row_index ? 1 : TOK,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
     CUtensorMap map_h = map, map_b = map;
     if (p.ids) {
-        encode_tensor_map_2d(&map_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, 64, 1,
+        encode_tensor_map_2d(&map_h, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, 64, 1,
                              CU_TENSOR_MAP_SWIZZLE_128B);
-        encode_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.b2, 2 * p.rank,
+        encode_tensor_map_2d(&map_b, f16, p.b2, 2 * p.rank,
                              static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank, 64, 128,
                              CU_TENSOR_MAP_SWIZZLE_128B);
     }
