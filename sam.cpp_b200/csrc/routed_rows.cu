@@ -47,7 +47,7 @@
 namespace samq {
 namespace {
 
-constexpr int kDecodeWarps = 16;
+constexpr int kDecodeWarps = 12;
 constexpr int kXWarp = 6 + kDecodeWarps;
 constexpr int kThreads = 32 * (kXWarp + 1);
 constexpr int kSets = kDecodeWarps / 4;

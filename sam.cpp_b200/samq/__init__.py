@@ -700,51 +700,80 @@ def neck_forward(neck: Neck, x, grid_w: int, grid_h: int, outs, stream=None):
 # ..._workspace() size, kept by a caller that calls often or captures a graph;
 # without one a call that needs memory takes it from torch's caching allocator.
 
+_elements = {}
+_torch = None  # torch, once a routed call has needed it (the binding itself does not)
+
+
+def _load_torch():
+    global _torch
+    import torch
+    _elements.update({torch.float16: F16, torch.float32: F32})
+    _torch = torch
+    return torch
+
+
 def _element(dtype) -> int:
     """F16 / F32 of a torch dtype (or the id itself)."""
     if isinstance(dtype, int):
         return dtype
-    name = str(dtype)
-    if name == "torch.float16":
-        return F16
-    if name == "torch.float32":
-        return F32
-    raise TypeError(f"float16 or float32 expected, got {name}")
+    if _torch is None:
+        _load_torch()
+    if dtype not in _elements:
+        raise TypeError(f"float16 or float32 expected, got {dtype}")
+    return _elements[dtype]
 
 
 def _same_device(device: int | None, *tensors) -> int:
-    """The one device of the given tensors (None entries skipped), which must be `device` where that is given."""
+    """The one CUDA device of the given tensors (None entries skipped), which must be `device` where that is given."""
     for t in tensors:
-        if t is None:
-            continue
-        if t.device.type != "cuda" or (device is not None and t.device.index != device):
-            raise ValueError(f"tensor on {t.device}, expected cuda:{'' if device is None else device}")
-        device = t.device.index
+        if t is not None:
+            d = t.get_device()  # -1 off the GPU
+            if d < 0 or (device is not None and d != device):
+                raise ValueError(f"tensor on {t.device}, expected cuda:{'' if device is None else device}")
+            device = d
     return device
 
 
 def _int32(*tensors):
+    int32 = (_torch or _load_torch()).int32
     for t in tensors:
-        if t is not None and str(t.dtype) != "torch.int32":
+        if t is not None and t.dtype is not int32:
             raise TypeError(f"index tensors are int32, got {t.dtype}")
+
+
+def _float32(*tensors):
+    float32 = (_torch or _load_torch()).float32
+    for t in tensors:
+        if t is not None and t.dtype is not float32:
+            raise TypeError(f"float32 expected, got {t.dtype}")
 
 
 def _stream_on(stream, device: int):
     if stream is None:
-        import torch
-        return torch.cuda.current_stream(device).cuda_stream
+        return (_torch or _load_torch())._C._cuda_getCurrentRawStream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _call_on(device: int, function, *args):
+    """A call that runs on the current device, with `device` made current where it is not."""
+    torch = _torch or _load_torch()
+    if torch._C._cuda_getDevice() == device:
+        status = function(*args)
+    else:
+        with torch.cuda.device(device):
+            status = function(*args)
+    if status:
+        _check(status)
 
 
 def _scratch(workspace, needed: int, device: int):
     """(tensor kept alive by the caller, address, bytes) of a workspace."""
-    if workspace is None and needed:
-        import torch
-        workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
     if workspace is None:
-        return None, None, 0
+        if not needed:
+            return None, None, 0
+        workspace = (_torch or _load_torch()).empty(needed, dtype=_torch.uint8, device=f"cuda:{device}")
     _same_device(device, workspace)
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace, workspace.data_ptr(), workspace.nbytes
 
 
 def route_workspace(tokens: int, experts: int, top_k: int) -> int:
@@ -754,17 +783,14 @@ def route_workspace(tokens: int, experts: int, top_k: int) -> int:
 def route(logits, tokens: int, experts: int, ld: int, top_k: int, weights, ids, offsets, rows, slots,
           normalize: bool = True, workspace=None, stream=None):
     """samq_route_v1: the top_k experts of every row of logits, their weights and the plan sorted by expert."""
-    import torch
     device = _same_device(None, logits, weights, ids, offsets, rows, slots)
     _int32(ids, offsets, rows, slots)
-    if logits.dtype != torch.float32 or weights.dtype != torch.float32:
-        raise TypeError("logits and weights are float32")
+    _float32(logits, weights)
     keep, address, size = _scratch(workspace, 0 if workspace is not None else route_workspace(tokens, experts, top_k),
                                    device)
-    with torch.cuda.device(device):
-        _check(library().samq_route_v1(logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0,
-                                       weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
-                                       slots.data_ptr(), address, size, _stream_on(stream, device)))
+    _call_on(device, library().samq_route_v1, logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0,
+             weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), address, size,
+             _stream_on(stream, device))
 
 
 def linear_grouped_workspace(w: Weights, groups: int, x_rows: int, rows: int, x_dtype, indexed: bool = True) -> int:
@@ -779,27 +805,28 @@ def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, r
     group g; w holds the groups' matrices stacked (w.n = groups * n)."""
     device = _same_device(w.device, x, offsets, y, row_index, bias)
     _int32(offsets, row_index)
+    _float32(bias)
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt,
                                                                             row_index is not None)
     keep, address, size = _scratch(workspace, needed, device)
-    _check(library().samq_linear_grouped_v1(w.handle, groups, x.data_ptr(), xt, x_rows, ldx, _addr(row_index),
-                                            offsets.data_ptr(), rows, _addr(bias), epilogue, y.data_ptr(), yt, ldy,
-                                            address, size, _stream_on(stream, device)))
+    status = library().samq_linear_grouped_v1(
+        w.handle, groups, x.data_ptr(), xt, x_rows, ldx, None if row_index is None else row_index.data_ptr(),
+        offsets.data_ptr(), rows, None if bias is None else bias.data_ptr(), epilogue, y.data_ptr(), yt, ldy, address,
+        size, _stream_on(stream, device))
+    if status:
+        _check(status)
 
 
 def combine(y, y_rows: int, ldy: int, slots, weights, tokens: int, top_k: int, width: int, out, ldo: int,
             residual=None, ldr: int = 0, stream=None):
     """samq_combine_v1: out[t] = residual[t] + sum_j weights[t][j] y[slots[t][j]]."""
-    import torch
     device = _same_device(None, y, slots, weights, out, residual)
     _int32(slots)
-    if any(t is not None and t.dtype != torch.float32 for t in (weights, out, residual)):
-        raise TypeError("weights, residual and out are float32")
-    with torch.cuda.device(device):
-        _check(library().samq_combine_v1(y.data_ptr(), _element(y.dtype), y_rows, ldy, slots.data_ptr(),
-                                         weights.data_ptr(), tokens, top_k, width, _addr(residual), ldr,
-                                         out.data_ptr(), ldo, _stream_on(stream, device)))
+    _float32(weights, out, residual)
+    _call_on(device, library().samq_combine_v1, y.data_ptr(), _element(y.dtype), y_rows, ldy, slots.data_ptr(),
+             weights.data_ptr(), tokens, top_k, width, None if residual is None else residual.data_ptr(), ldr,
+             out.data_ptr(), ldo, _stream_on(stream, device))
 
 
 class Adapters:
@@ -847,9 +874,12 @@ def linear_adapters(w: Weights, adapters: Adapters, x, m: int, ldx: int, ids, y,
     range)."""
     device = _same_device(w.device, x, ids, y, bias)
     _int32(ids)
+    _float32(bias)
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_adapters_workspace(w, adapters, m, xt)
     keep, address, size = _scratch(workspace, needed, device)
-    _check(library().samq_linear_adapters_v1(w.handle, adapters.handle, x.data_ptr(), xt, m, ldx, ids.data_ptr(),
-                                             _addr(bias), epilogue, y.data_ptr(), yt, ldy, address, size,
-                                             _stream_on(stream, device)))
+    status = library().samq_linear_adapters_v1(
+        w.handle, adapters.handle, x.data_ptr(), xt, m, ldx, ids.data_ptr(), None if bias is None else bias.data_ptr(),
+        epilogue, y.data_ptr(), yt, ldy, address, size, _stream_on(stream, device))
+    if status:
+        _check(status)
