@@ -15,7 +15,7 @@ namespace {
 // (zeros for an index outside [0, x_rows)), f32 rows staged by the Q8_1 rule on
 // the way.  A thread moves 8 columns; four neighbouring threads a 32-value block.
 // Bound by memory: 2 + 2 (f16) or 4 + 2 (f32) bytes an element.
-template <class T>
+template <class T, int U>
 __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ x, int64_t x_rows, int64_t ldx,
                                                           const int* __restrict__ row_index, int64_t rows, int k,
                                                           __half* __restrict__ out, DeviceStatus* status) {
@@ -24,29 +24,40 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ 
     const uint32_t per_row = static_cast<uint32_t>(k / 8);
     const int64_t units = rows * per_row;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-    // Whole warps: a unit's block neighbours are lanes of the same warp.
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u - (threadIdx.x & 31) < units;
-         u += stride) {
-        const int64_t row = u < units ? u / per_row : 0;
-        const int c = static_cast<int>(u - row * per_row) * 8;
-        const int64_t src = u < units ? __ldg(row_index + row) : -1;
-        const bool in = src >= 0 && src < x_rows;
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if constexpr (sizeof(T) == 2) {
-            if (in) o = __ldg(reinterpret_cast<const uint4*>(x + src * ldx + c));
-        } else {
-            float v[8] = {};
-            if (in) {
-                const float4 a = __ldg(reinterpret_cast<const float4*>(x + src * ldx + c));
-                const float4 b = __ldg(reinterpret_cast<const float4*>(x + src * ldx + c) + 1);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-            }
-            uint32_t pair[4];
-            record_range(stage_q8_1<4, 8>(v, pair), status);
-            o = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+    // Whole warps: a unit's block neighbours are lanes of the same warp.  A thread asks for U units at once.
+    for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u0 - (threadIdx.x & 31) < units;
+         u0 += U * stride) {
+        int64_t src[U];
+        int c[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t u = u0 + i * stride;
+            const int64_t row = u < units ? u / per_row : 0;
+            c[i] = static_cast<int>(u - row * per_row) * 8;
+            src[i] = u < units ? __ldg(row_index + row) : -1;
+            if (src[i] >= x_rows) src[i] = -1;
         }
-        if (u < units) *reinterpret_cast<uint4*>(out + u * 8) = o;
+        constexpr int W = sizeof(T) == 2 ? 1 : 2;
+        uint4 raw[U][W];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                raw[i][j] = src[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(x + src[i] * ldx + c[i]) + j)
+                                        : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t u = u0 + i * stride;
+            uint4 o = raw[i][0];
+            if constexpr (sizeof(T) == 4) {
+                const float* f = reinterpret_cast<const float*>(raw[i]);
+                const float v[8] = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+                uint32_t pair[4];
+                record_range(stage_q8_1<4, 8>(v, pair), status);
+                o = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+            }
+            if (u < units) *reinterpret_cast<uint4*>(out + u * 8) = o;
+        }
     }
 }
 
@@ -54,14 +65,19 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ 
 
 void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index, int64_t rows,
                         int k, __half* out, DeviceState& state, cudaStream_t stream) {
+    // Units per thread: several where there is work for the whole GPU all the same.
     const int64_t blocks = (rows * (k / 8) + 255) / 256;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(state.sm_count) * 32)));
+    const bool many = blocks >= 16 * state.sm_count;
+    const int64_t wanted = many ? (blocks + 3) / 4 : blocks;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(wanted, static_cast<int64_t>(state.sm_count) * 64)));
+    const __half* xh = static_cast<const __half*>(x);
+    const float* xf = static_cast<const float*>(x);
     if (x_type == SAMQ_TYPE_F16)
-        launch_pdl(gather_rows_kernel<__half>, grid, dim3(256), 0, stream, "gather_rows_kernel launch",
-                   static_cast<const __half*>(x), x_rows, ldx, row_index, rows, k, out, state.status);
+        launch_pdl(many ? gather_rows_kernel<__half, 4> : gather_rows_kernel<__half, 1>, grid, dim3(256), 0, stream,
+                   "gather_rows_kernel launch", xh, x_rows, ldx, row_index, rows, k, out, state.status);
     else
-        launch_pdl(gather_rows_kernel<float>, grid, dim3(256), 0, stream, "gather_rows_kernel launch",
-                   static_cast<const float*>(x), x_rows, ldx, row_index, rows, k, out, state.status);
+        launch_pdl(many ? gather_rows_kernel<float, 4> : gather_rows_kernel<float, 1>, grid, dim3(256), 0, stream,
+                   "gather_rows_kernel launch", xf, x_rows, ldx, row_index, rows, k, out, state.status);
 }
 
 // Few rows stream the packets, many take the f16 tiles.  Between, a call holds

@@ -106,10 +106,11 @@ __device__ __forceinline__ int clamp_row(int v, int64_t rows) {
 
 struct Tile {
     int group, row0, end, col0;  // plan rows row0 .. end - 1, columns col0 ..
+    bool narrow;                 // half the tile's columns or fewer: half the MMA
 };
 
 // The groups' tiles in order: s_first[g] is the number of row tiles before group g.
-__device__ __forceinline__ Tile find_tile(int tile, int n_tiles, int bn, int rows_per_tile, int groups,
+__device__ __forceinline__ Tile find_tile(int tile, int n_tiles, int n, int bn, int rows_per_tile, int groups,
                                           const int* s_first, const int* s_begin, const int* s_end) {
     const int rt = tile / n_tiles;
     int lo = 0, hi = groups;  // s_first[lo] <= rt < s_first[hi]
@@ -123,6 +124,7 @@ __device__ __forceinline__ Tile find_tile(int tile, int n_tiles, int bn, int row
     t.row0 = s_begin[lo] + (rt - s_first[lo]) * rows_per_tile;
     t.end = s_end[lo];
     t.col0 = (tile - rt * n_tiles) * bn;
+    t.narrow = n - t.col0 <= bn / 2;
     return t;
 }
 
@@ -218,7 +220,6 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         bool ok = true;
         const int no_row = static_cast<int>(p.rows);  // an index that reads zeros
         const uint32_t full_bar = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);  // the even CTA's
-        const int b_half = rank * (BN / CTAS);
         // The whole warp waits for the next stage; one thread of the X warp announces the step.
         auto open = [&](bool last) -> bool {
             if (!mbar_wait_warp(&empty[s], ph ^ 1u, status, 61)) return false;
@@ -238,8 +239,9 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             }
         };
         for (int tile = unit; tile < tiles && ok; tile += units) {
-            const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
+            const Tile t = find_tile(tile, n_tiles, p.n, BN, kTileRows, p.groups, s_first, s_begin, s_end);
             const int row0 = t.row0 + rank * BM;
+            const int b_half = rank * (t.narrow ? BN / 2 : BN) / CTAS;
             const int mine = row0 + 4 * lane;  // this lane's four rows of the CTA's 128
             // The pair's 256 rows hold the same adapters for both CTAs.
             int own[4], other[4];
@@ -318,7 +320,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            constexpr uint32_t idesc = idesc_f16_f32(CTAS * BM, BN);
+            constexpr uint32_t idesc_full = idesc_f16_f32(CTAS * BM, BN), idesc_half = idesc_f16_f32(CTAS * BM, BN / 2);
             // Descriptors of stage 0; a stage or 32 bytes on only moves the address field (16-byte units).
             const uint64_t a_desc = smem_desc_sw128(smem_u32(sa)), b_desc = smem_desc_sw128(smem_u32(sb));
             int s = 0;
@@ -339,6 +341,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 if (!free) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kAccStride);
+                const uint32_t idesc = p.n - tile % n_tiles * BN <= BN / 2 ? idesc_half : idesc_full;
                 uint32_t accumulate = 0;
                 bool last = false;
                 while (!last) {
@@ -389,7 +392,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         int acc = 0;
         uint32_t acc_ph = 0;
         for (int tile = unit; tile < tiles; tile += units) {
-            const Tile t = find_tile(tile, n_tiles, BN, kTileRows, p.groups, s_first, s_begin, s_end);
+            const Tile t = find_tile(tile, n_tiles, p.n, BN, kTileRows, p.groups, s_first, s_begin, s_end);
             const int row0 = t.row0 + rank * BM + quarter * 32;
             const float* bias = p.bias ? p.bias + static_cast<int64_t>(t.group) * p.n + t.col0 : nullptr;
             const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15u) == 0;
@@ -427,7 +430,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                     for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(r[i]);
                     if (p.gelu) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = gelu_erf(v[i]);
+                        for (int i = 0; i < 32; i += 2) gelu_erf2(v[i], v[i + 1]);
                     }
                     // 16-byte unit u of row `lane` at u ^ (lane % 8): the store's 128-byte swizzle.
                     if (f16) {

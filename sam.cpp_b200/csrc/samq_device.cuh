@@ -247,6 +247,52 @@ __device__ __forceinline__ float gelu_erf(float x) {
     return x * (x >= 0.0f ? 1.0f - q : q);
 }
 
+// ---- pairs of floats: one instruction for two f32 operations ----------------
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+
+// gelu_erf of two values with packed arithmetic.  The last step is
+// max(x, 0) - |x| q, which is x (1 - q) for x >= 0 and x q for x < 0; |x| is
+// bounded there, as an infinite one has q = 0.
+__device__ __forceinline__ void gelu_erf2(float& x0, float& x1) {
+    constexpr float b1 = 0.127414796f, b2 = -0.142248368f, b3 = 0.7107068705f, b4 = -0.7265760135f,
+                    b5 = 0.5307027145f, p = 0.3275911f * 0.70710678118654752f;
+    const uint64_t a = pack2(fminf(fabsf(x0), 1e30f), fminf(fabsf(x1), 1e30f)), x = pack2(x0, x1);
+    float d0, d1;
+    unpack2(fma2(a, pack2(p, p), pack2(1.0f, 1.0f)), d0, d1);
+    const uint64_t t = pack2(rcp_mufu(d0), rcp_mufu(d1));
+    uint64_t poly = fma2(pack2(b5, b5), t, pack2(b4, b4));
+    poly = fma2(poly, t, pack2(b3, b3));
+    poly = fma2(poly, t, pack2(b2, b2));
+    poly = fma2(poly, t, pack2(b1, b1));
+    poly = mul2(poly, t);
+    float e0, e1;
+    unpack2(mul2(mul2(x, x), pack2(-0.72134752044448170f, -0.72134752044448170f)), e0, e1);
+    const uint64_t q = mul2(poly, pack2(ex2_mufu(e0), ex2_mufu(e1)));
+    unpack2(fma2(mul2(a, pack2(-1.0f, -1.0f)), q, pack2(fmaxf(x0, 0.0f), fmaxf(x1, 0.0f))), x0, x1);
+}
+
 // ---- programmatic dependent launch ---------------------------------------
 // Kernels launched with cudaLaunchAttributeProgrammaticStreamSerialization may
 // start before the previous kernel on the stream has finished; each of them

@@ -420,7 +420,7 @@ void launch_route(const float* logits, int64_t tokens, int experts, int64_t ld, 
                   DeviceState& state, cudaStream_t stream);
 void launch_combine(const void* y, int y_type, int64_t y_rows, int64_t ldy, const int32_t* slots, const float* weights,
                     int64_t tokens, int top_k, int64_t width, const float* residual, int64_t ldr, float* out,
-                    int64_t ldo, DeviceState& state, cudaStream_t stream);
+                    int64_t ldo, cudaStream_t stream);
 
 // grouped.cu: products whose weight depends on the row.
 struct RoutedProduct {
