@@ -14,7 +14,7 @@
 // one launch, no atomics, no workspace.
 //
 // One CTA per SM, persistent over the units of all groups:
-//   warp 0       packets, kLoad contiguous ones by one bulk copy, then 128 x 64 of
+//   warp 0       packets, kDepth contiguous ones by one bulk copy, then 128 x 64 of
 //                B | B by TMA for each adapter step;
 //   last warp    the same columns of X by TMA (rows by index through the row gather),
 //                hi | lo of the adapter's rows by the row gather;
@@ -22,7 +22,7 @@
 //   warps 2-5    epilogue: one weight row a lane, TMEM to registers (SPLIT > 1: to
 //                shared memory of the CTA that adds up the row), bias, erf-GELU,
 //                stores coalesced over the weight rows;
-//   warps 6-     decoders, sets of four on steps of kDepth packets in turn: a thread
+//   warps 6-     decoders, sets of four on steps of several packets in turn: a thread
 //                turns a row of its packets into f16 with the values of packets.cuh bit
 //                for bit and stores it to tensor memory, where the MMA takes it as its
 //                left factor.
@@ -51,8 +51,6 @@ constexpr int kDecodeWarps = 12;
 constexpr int kXWarp = 6 + kDecodeWarps;
 constexpr int kThreads = 32 * (kXWarp + 1);
 constexpr int kSets = kDecodeWarps / 4;
-constexpr int kDepth = 2;               // packets (64 columns each) of a step
-constexpr int kTmemStep = 32 * kDepth;  // TMEM columns of a step's left factor: 128 rows x 64 kDepth f16
 constexpr int kMaxGroups = 1024;
 constexpr int kSmemLimit = 232448;
 constexpr int kMaxSplit = 8;
@@ -61,19 +59,20 @@ constexpr int kMaxChunks = kRoutedFewAdapted / 64;  // row chunks of a call with
 template <int TYPE, int TOK>
 struct RowsSmem {
     static constexpr int packet = 128 * (code_bytes_of(TYPE) + 8);
-    static constexpr int load = TOK == 64 ? 2 : 4;  // packets of a copy
-    static constexpr int raw_bytes = load * packet;
+    static constexpr int depth = TOK == 64 ? 2 : 4;  // packets (64 columns each) of a copy and of a step
+    static constexpr int slot = 32 * depth;          // TMEM columns of a step's left factor: 128 rows x 64 depth f16
+    static constexpr int raw_bytes = depth * packet;
     static constexpr int b_bytes = 128 * 128;  // an adapter step's B | B, where the packets lie
     static constexpr int raw_stage = (raw_bytes > b_bytes ? raw_bytes : b_bytes + 1023) / 1024 * 1024;
     static constexpr int x_chunk = TOK * 128;  // 64 columns of TOK rows
-    static constexpr int x_bytes = load * x_chunk;
+    static constexpr int x_bytes = depth * x_chunk;
     static constexpr int part = TOK * 128 * 4;  // partial sums [TOK][128]
     static constexpr int tables = (3 * kMaxGroups + 1) * 4;
     static constexpr int lists = kMaxChunks * (TOK + 1) * 4;  // the adapters of each row chunk and how many
     static constexpr int fixed = 1024 + part + 512 + tables + lists;
     static constexpr int fit = (kSmemLimit - fixed) / (raw_stage + x_bytes);
     static constexpr int stages = fit > 8 ? 8 : fit;
-    static constexpr int slots = (512 - 2 * TOK) / kTmemStep < 8 ? (512 - 2 * TOK) / kTmemStep : 8;  // left factors
+    static constexpr int slots = (512 - 2 * TOK) / slot;  // left factors
     static constexpr int raw_off = stages * x_bytes;
     static constexpr int part_off = raw_off + stages * raw_stage;
     static constexpr int bar_off = part_off + part;
@@ -255,8 +254,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                    const __grid_constant__ CUtensorMap map_b, const RoutedProduct p, int max_rows, int split,
                    DeviceStatus* status) {
     using L = RowsSmem<TYPE, TOK>;
-    constexpr int kStages = L::stages, kSlots = L::slots, kLoad = L::load;
-    constexpr int kSteps = kLoad / kDepth;  // of a copy
+    constexpr int kStages = L::stages, kSlots = L::slots, kDepth = L::depth, kTmemStep = L::slot;
     static_assert(kStages >= 2 && kSlots >= kSets && L::total <= kSmemLimit, "shared memory budget");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -366,7 +364,6 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int units = s_first[p.groups];
-    const int loads = (steps + kSteps - 1) / kSteps;  // copies of a unit's packets
     // A unit's steps of this rank: `steps` of packets, then adapter steps rank, rank + split, ... of the
     // chunk's adapters x the 64-column pieces of their pair.
     const int pieces = p.ids ? (2 * p.rank + 63) / 64 : 0;
@@ -396,9 +393,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     const int left = min(chunks - step0 * kDepth, steps * kDepth);
                     const uint8_t* from =
                         p.packets + (static_cast<int64_t>(u.tile) * chunks + step0 * kDepth) * L::packet;
-                    for (int c = 0; c < left; c += kLoad) {
+                    for (int c = 0; c < left; c += kDepth) {
                         if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
-                        const int bytes = min(kLoad, left - c) * L::packet;
+                        const int bytes = min(kDepth, left - c) * L::packet;
                         mbar_arrive_expect_tx(&full[s], bytes);
                         bulk_load_1d(sraw + s * L::raw_stage, from, bytes, &full[s]);
                         from += L::raw_bytes;
@@ -418,13 +415,13 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             } else {
                 if (!p.row_index) {
                     if (elect_one())
-                        for (int c = step0 * kDepth; c < min(chunks, (step0 + steps) * kDepth); c += kLoad) {
+                        for (int c = step0 * kDepth; c < min(chunks, (step0 + steps) * kDepth); c += kDepth) {
                             if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
                             if (p.k % 64 == 0) {  // one copy; the chunks past the end read zeros
                                 mbar_arrive_expect_tx(&full[s], L::x_bytes);
                                 tma_load_3d(sx + s * L::x_bytes, &map_x, &full[s], 0, u.row0, c);
                             } else {
-                                const int here = min(kLoad, chunks - c);
+                                const int here = min(kDepth, chunks - c);
                                 mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
                                 for (int j = 0; j < here; ++j)
                                     tma_load_2d(sx + s * L::x_bytes + j * L::x_chunk, &map_x, &full[s], (c + j) * 64,
@@ -435,9 +432,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     __syncwarp();
                 }
                 // Rows by index and adapter rows: four rows a lane.
-                const int first = p.row_index ? 0 : loads;
+                const int first = p.row_index ? 0 : steps;
                 ok = __all_sync(0xffffffffu, ok);
-                if (ok && first < loads + more) {
+                if (ok && first < steps + more) {
                     int rows[4], id[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -450,13 +447,12 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     if (more) pdl_wait();  // the pairs of the down product
                     s = (before + first) % kStages;
                     ph = static_cast<uint32_t>((before + first) / kStages) & 1u;
-                    for (int i = first; i < loads + more; ++i) {
+                    for (int i = first; i < steps + more; ++i) {
                         if (elect_one()) ok = mbar_wait(&empty[s], ph ^ 1u, status, 71);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
-                        if (i < loads) {
-                            const int c0 = step0 * kDepth + i * kLoad;
-                            const int here = min(kLoad, min(chunks, (step0 + steps) * kDepth) - c0);
+                        if (i < steps) {
+                            const int c0 = (step0 + i) * kDepth, here = min(kDepth, chunks - c0);
                             if (elect_one()) mbar_arrive_expect_tx(&full[s], here * L::x_chunk);
                             __syncwarp();
                             if (lane < TOK / 4)
@@ -464,7 +460,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                                     gather4(sx + s * L::x_bytes + c * L::x_chunk + lane * 512, &map_x, &full[s],
                                             (c0 + c) * 64, rows);
                         } else {
-                            const int at = rank + (i - loads) * split;
+                            const int at = rank + (i - steps) * split;
                             const int a = s_list[u.chunk * TOK + at / pieces];
                             if (elect_one()) mbar_arrive_expect_tx(&full[s], L::x_chunk);
                             __syncwarp();
@@ -481,7 +477,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
-            before += loads + more;
+            before += steps + more;
         }
         if (is_x) pdl_wait();  // if not before: the kernel ends after its predecessors
         pdl_trigger();  // this warp's loads are issued
@@ -509,15 +505,13 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * TOK);
                 for (int i = 0; i < steps; ++i) {
-                    const int part = i % kSteps;  // of its copy
-                    if ((part == 0 && !mbar_wait(&full[s], ph, status, 73)) ||
-                        !mbar_wait(&a_full[slot], slot_ph, status, 74)) {
+                    if (!mbar_wait(&full[s], ph, status, 73) || !mbar_wait(&a_full[slot], slot_ph, status, 74)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t a = tmem_base + kTmemA + static_cast<uint32_t>(slot * kTmemStep);
-                    const uint64_t xd = x_desc + static_cast<uint32_t>((s * L::x_bytes + part * kDepth * L::x_chunk) >> 4);
+                    const uint64_t xd = x_desc + static_cast<uint32_t>(s * (L::x_bytes >> 4));
                     const int here = min(kDepth, chunks - (step0 + i) * kDepth);
 #pragma unroll
                     for (int c = 0; c < kDepth; ++c)
@@ -531,10 +525,8 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                         slot = 0;
                         slot_ph ^= 1u;
                     }
-                    if (part == kSteps - 1 || i == steps - 1) {
-                        tc_commit(&empty[s]);
-                        advance();
-                    }
+                    tc_commit(&empty[s]);
+                    advance();
                 }
                 const int more = ok && p.ids ? adapter_steps(unit / group_tiles(0, p.n)) : 0;
                 for (int i = 0; i < more; ++i) {
@@ -573,7 +565,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             int i = set - done % kSets;
             if (i < 0) i += kSets;  // this set's first step of the unit
             for (; i < steps; i += kSets) {
-                const int copy = copies + i / kSteps, s = copy % kStages;
+                const int copy = copies + i, s = copy % kStages;
                 const int step = done + i, slot = step % kSlots;
                 ok = __all_sync(0xffffffffu,
                                 mbar_wait(&full[s], static_cast<uint32_t>(copy / kStages) & 1u, status, 77) &&
@@ -582,7 +574,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 tc_fence_after();
                 const int here = min(kDepth, chunks - (step0 + i) * kDepth);
                 for (int c = 0; c < here; ++c) {
-                    const uint8_t* raw = sraw + s * L::raw_stage + (i % kSteps * kDepth + c) * L::packet;
+                    const uint8_t* raw = sraw + s * L::raw_stage + c * L::packet;
                     uint32_t w[32];
                     decode_row<TYPE>(raw + r * code_bytes_of(TYPE), raw + 128 * code_bytes_of(TYPE) + r * 8, magic, w);
                     tc_st_32x32b_x32(lanes + static_cast<uint32_t>(slot * kTmemStep + 32 * c), w);
@@ -593,7 +585,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 if (lane == 0) mbar_arrive(&a_full[slot]);
             }
             done += steps;
-            copies += loads;
+            copies += steps;
             if (p.ids) copies += adapter_steps(unit / group_tiles(0, p.n));  // one group
         }
     } else {
@@ -723,7 +715,7 @@ void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStre
     CUtensorMap map;
     const auto f16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (!p.row_index && p.k % 64 == 0)  // [k / 64][x_rows][64]: several 64-column chunks a copy
-        encode_tensor_map_3d_box(&map, f16, p.x, 64, p.x_rows, p.k / 64, p.ldx * 2, 128, 64, TOK, L::load,
+        encode_tensor_map_3d_box(&map, f16, p.x, 64, p.x_rows, p.k / 64, p.ldx * 2, 128, 64, TOK, L::depth,
                                  CU_TENSOR_MAP_SWIZZLE_128B);
     else
         encode_tensor_map_2d(&map, f16, p.x, p.k, p.x_rows, p.ldx * 2, 64, p.row_index ? 1 : TOK,
@@ -741,7 +733,7 @@ void run_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStre
                         "cudaFuncSetAttribute(routed rows smem)");
     const int tiles = (p.n + 127) / 128 + (p.n % 128 ? 1 : 0);  // of a group, at most
     const int64_t units = std::min<int64_t>(p.rows, p.groups + p.rows / TOK) * tiles;  // at most
-    const int steps = ((p.k + 63) / 64 + kDepth - 1) / kDepth;
+    const int steps = ((p.k + 63) / 64 + L::depth - 1) / L::depth;
     const void* fn = reinterpret_cast<const void*>(kernel);
     // Few units: the widest cluster that still has every unit resident.
     int split = 1;
