@@ -592,6 +592,8 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         const int quarter = warp & 3;  // TMEM lanes 32 * quarter ..
         const int mine = quarter * 32 + lane;
         const bool f16 = p.y_type == SAMQ_TYPE_F16;
+        const int elem = f16 ? 2 : 4;
+        const int64_t stride = p.ldy * elem;
         const int shift = 31 - __clz(split);  // split is a power of two
         const int share = TOK >> shift;       // rows that a CTA of the cluster finishes: t % split == rank
         int acc = 0;
@@ -614,14 +616,20 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             // This lane's weight row as a column of the group's output.
             const int64_t col = static_cast<int64_t>(u.tile) * 128 + mine - static_cast<int64_t>(u.group) * p.n;
             const bool in = col >= 0 && col < p.n;
-            const int64_t at0 = u.row0 * p.ldy + col;
-            auto finish = [&](int t, float v) {
-                v += bias;
-                if (p.gelu) v = gelu_erf(v);
+            uint8_t* out = static_cast<uint8_t*>(p.y) + (u.row0 * p.ldy + col) * elem;
+            // Rows t and t + step (where `both`): their sums a and b through the epilogue and out.
+            auto finish = [&](int t, int step, bool both, float a, float b) {
+                a += bias;
+                b += bias;
+                if (p.gelu) gelu_erf2(a, b);
+                uint8_t* at = out + t * stride;
                 if (!in) return;
-                const int64_t at = at0 + t * p.ldy;
-                if (f16) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
-                else static_cast<float*>(p.y)[at] = v;
+                if (f16) *reinterpret_cast<__half*>(at) = __float2half_rn(a);
+                else *reinterpret_cast<float*>(at) = a;
+                if (!both) return;
+                at += step * stride;
+                if (f16) *reinterpret_cast<__half*>(at) = __float2half_rn(b);
+                else *reinterpret_cast<float*>(at) = b;
             };
             // Warp-uniform: the TMEM loads below are warp-collective.
             if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_ph, status, 79))) break;
@@ -648,8 +656,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < C; ++i)
-                        if (c + i < u.count) finish(c + i, __uint_as_float(v[i]));
+                    for (int i = 0; i < C; i += 2) {
+                        if (c + i >= u.count) break;
+                        finish(c + i, 1, c + i + 1 < u.count, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                    }
                 }
                 __syncwarp();  // converged for the next collective load
             }
@@ -661,11 +671,15 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             if (split > 1) {
                 if (lane < split) mbar_arrive_cluster(cluster_map(part_full, lane));
                 if (!__all_sync(0xffffffffu, mbar_wait_cluster(part_full, part_ph, status, 81))) break;
-                for (int t = rank; t < u.count; t += split) {
+                for (int t = rank; t < u.count; t += 2 * split) {
+                    const bool both = t + split < u.count;
                     const float* from = spart + (t >> shift) * 128 + mine;
-                    float v = 0.0f;
-                    for (int o = 0; o < split; ++o) v += from[o * share * 128];
-                    finish(t, v);
+                    float v0 = 0.0f, v1 = 0.0f;
+                    for (int o = 0; o < split; ++o) {
+                        v0 += from[o * share * 128];
+                        if (both) v1 += from[o * share * 128 + 128];
+                    }
+                    finish(t, split, both, v0, v1);
                 }
                 __syncwarp();
                 if (lane < split) mbar_arrive_cluster(cluster_map(part_free, lane));
