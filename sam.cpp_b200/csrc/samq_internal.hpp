@@ -452,8 +452,15 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
                          cudaStream_t stream);
 void launch_routed(const RoutedProduct& p, DeviceState& state, cudaStream_t stream);
-constexpr int kRoutedFewRows = 64;      // rows of a group, at most, that take the packet-streaming kernel
-constexpr int kRoutedFewAdapted = 256;  // the same for a call with adapters
+// Which kernels a product of `rows` rows over `groups` groups of n x k weights runs.
+enum class RoutedPath {
+    kRows,   // routed_rows.cu alone: any group, its weights decoded once for every few rows
+    kTiles,  // routed_tile.cu alone
+    kBoth    // groups of at most kRoutedFewRows rows by the first, the others by the second
+};
+constexpr int kRoutedFewRows = 64;
+constexpr int kRoutedFewAdapted = 256;  // rows of a call with adapters, at most, that routed_rows.cu takes
+RoutedPath routed_path(int64_t rows, int groups, int64_t n, int64_t k, bool adapted);
 // routed_rows.cu: the groups of at most `max_rows` rows from their packets.
 void launch_routed_rows(const RoutedProduct& p, int max_rows, DeviceState& state, cudaStream_t stream);
 // routed_tile.cu: the groups of at least `min_rows` rows on tensor-core tiles.
