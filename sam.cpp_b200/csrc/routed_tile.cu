@@ -5,11 +5,11 @@
 // Mathematics.  One tile is D = X_tile . W_tile^T over k, in f32 in TMEM.  The
 // adapters ride on the same accumulator as more depth:
 //   delta_i = B_a h_i, h_i = scale_a A_a x_i (a = ids[i]),
-//   D += [hi(H) | lo(H)]_a . [B_a | B_a]^T for every adapter a with rows in the tile,
-// where row i of the left factor is h_i's f16 pair if ids[i] == a and zero
-// otherwise.  The zero rows cost nothing to make: the left factor is a TMA
-// gather by row index, and an index past the end reads zeros.  The pair keeps h
-// to 2^-22, f32's level against the f16 rounding of B.
+//   D += [hi(H) | lo(H)] . [B_a | B_a]^T for every adapter a with rows in the tile,
+// on the accumulator rows i with ids[i] == a alone: the MMA leaves the lanes of the
+// others as they are.  The pair keeps h to 2^-22, f32's level against the f16
+// rounding of B.  (Zeroing the other rows of the left factor by a TMA row gather
+// instead made such a step 1.2 us, three times a step of W.)
 //
 // x arrives in plan order: a row_index has been applied by gather_rows_kernel.
 // Gathering inside this kernel was measured and not kept (10368 rows of 8
@@ -57,12 +57,12 @@ struct TileSmem {
     static constexpr int stage = a_bytes + b_bytes;
     static constexpr int out = kEpilogueWarps * kSlabBytes;
     static constexpr int tables = (3 * GROUPS + 1) * 4;  // begin, end, tile prefix of each group
-    static constexpr int fixed = 1024 + out + tables + 256;
+    static constexpr int fixed = 1024 + out + tables + 512;
     static constexpr int stages = (kSmemLimit - fixed) / stage > 8 ? 8 : (kSmemLimit - fixed) / stage;
     static constexpr int b_off = stages * a_bytes;
     static constexpr int out_off = stages * stage;
     static constexpr int bar_off = out_off + out;
-    static constexpr int table_off = bar_off + 256;
+    static constexpr int table_off = bar_off + 512;
     static constexpr int total = stages * stage + fixed;
 };
 
@@ -70,28 +70,9 @@ struct TileMaps {
     CUtensorMap x;       // box 64 x 128
     CUtensorMap w;       // box 64 x BN / CTAS
     CUtensorMap h;       // adapters: [rows][2 rank], box 64 x 128
-    CUtensorMap h_rows;  // the same, box 64 x 1, gathered
     CUtensorMap b;       // adapters: [adapters * n][2 rank], box 64 x BN / CTAS
     CUtensorMap y;       // output, box 128 bytes x 32
 };
-
-// Four rows of 64 columns by index into shared memory (the map's box is one row
-// high).  CTAS == 2: `bar` is the shared::cluster address of either CTA's barrier.
-template <int CTAS>
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int x, int4 r) {
-    if constexpr (CTAS == 1)
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-            "%4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-            : "memory");
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
-            "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-            : "memory");
-}
 
 template <int CTAS>
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* local, uint32_t bar, int x,
@@ -134,7 +115,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
     using L = TileSmem<CTAS, BN, GROUPS>;
     constexpr int kStages = L::stages;
     static_assert(kStages >= 3 && L::total <= kSmemLimit, "shared memory budget");
-    static_assert(2 * 8 * kStages + 5 * 8 + 8 + 4 * kStages <= 256, "barrier space");
+    static_assert(2 * 8 * kStages + 5 * 8 + 8 + 36 * kStages <= 512, "barrier space");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sa = smem;
@@ -148,7 +129,10 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    volatile int* last_step = reinterpret_cast<int*>(tmem_slot + 2);
+    // Of each stage: kLast | kMasked, and the accumulator lanes an adapter step leaves alone.
+    constexpr int kLast = 1, kMasked = 2;
+    volatile int* step_kind = reinterpret_cast<int*>(tmem_slot + 2);
+    volatile uint32_t* step_off = tmem_slot + 2 + kStages;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CTAS == 2 ? static_cast<int>(cluster_cta_rank()) : 0;
@@ -218,13 +202,16 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
         uint32_t ph = 0;
         uint32_t issued = 0, issued_phase = 0;
         bool ok = true;
-        const int no_row = static_cast<int>(p.rows);  // an index that reads zeros
         const uint32_t full_bar = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);  // the even CTA's
         // The whole warp waits for the next stage; one thread of the X warp announces the step.
-        auto open = [&](bool last) -> bool {
+        auto open = [&](int kind, const uint32_t* off) -> bool {
             if (!mbar_wait_warp(&empty[s], ph ^ 1u, status, 61)) return false;
             if (is_x && rank == 0 && elect_one()) {
-                last_step[s] = last;
+                step_kind[s] = kind;
+                if (kind & kMasked) {
+#pragma unroll
+                    for (int j = 0; j < 4 * CTAS; ++j) step_off[8 * s + j] = off[j];
+                }
                 mbar_arrive_expect_tx(&full[s], CTAS * L::stage);
             }
             __syncwarp();
@@ -242,25 +229,22 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             const Tile t = find_tile(tile, n_tiles, p.n, BN, kTileRows, p.groups, s_first, s_begin, s_end);
             const int row0 = t.row0 + rank * BM;
             const int b_half = rank * (t.narrow ? BN / 2 : BN) / CTAS;
-            const int mine = row0 + 4 * lane;  // this lane's four rows of the CTA's 128
-            // The pair's 256 rows hold the same adapters for both CTAs.
-            int own[4], other[4];
+            // The adapters of the tile's rows (a pair's 256 for both CTAs): rows 32 j + lane.
+            int id[4 * CTAS];
             int next = p.adapter_count;
             if (p.ids) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    own[j] = mine + j < t.end ? __ldg(p.ids + mine + j) : -1;
-                    const int o = CTAS == 2 ? (rank ? mine + j - BM : mine + j + BM) : mine + j;
-                    other[j] = o < t.end ? __ldg(p.ids + o) : -1;
-                    if (own[j] >= 0) next = min(next, own[j]);
-                    if (other[j] >= 0) next = min(next, other[j]);
+                for (int j = 0; j < 4 * CTAS; ++j) {
+                    const int row = t.row0 + 32 * j + lane;
+                    id[j] = row < t.end ? __ldg(p.ids + row) : -1;
+                    if (id[j] >= 0) next = min(next, id[j]);
                 }
                 next = __reduce_min_sync(0xffffffffu, next);
             }
             const int wrow = t.group * p.n + t.col0 + b_half;
             const bool plain = next >= p.adapter_count;
             for (int kb = 0; kb < kblocks; ++kb) {
-                ok = open(kb == kblocks - 1 && plain);
+                ok = open(kb == kblocks - 1 && plain ? kLast : 0, nullptr);
                 if (!ok) break;
                 if (elect_one()) {
                     if (is_x)
@@ -276,24 +260,17 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
             while (ok && next < p.adapter_count) {
                 const int a = next;
                 next = p.adapter_count;
-                int v[4];
-                bool all = true;
+                uint32_t off[4 * CTAS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = own[j] == a ? mine + j : no_row;
-                    all &= own[j] == a || mine + j >= t.end;
-                    if (own[j] > a) next = min(next, own[j]);
-                    if (other[j] > a) next = min(next, other[j]);
+                for (int j = 0; j < 4 * CTAS; ++j) {
+                    off[j] = ~__ballot_sync(0xffffffffu, id[j] == a);
+                    if (id[j] > a) next = min(next, id[j]);
                 }
                 next = __reduce_min_sync(0xffffffffu, next);
-                all = __all_sync(0xffffffffu, all);  // no row to mask: a plain tile (rows past the end are not stored)
-                const int4 rows4 = make_int4(v[0], v[1], v[2], v[3]);
                 for (int c = 0; c < 2 * p.rank && ok; c += BK) {
-                    ok = open(c + BK >= 2 * p.rank && next >= p.adapter_count);
+                    ok = open(kMasked | (c + BK >= 2 * p.rank && next >= p.adapter_count ? kLast : 0), off);
                     if (!ok) break;
-                    if (is_x && !all) {
-                        tma_gather4<CTAS>(sa + s * L::a_bytes + lane * 512, &maps.h_rows, full_bar + 8 * s, c, rows4);
-                    } else if (elect_one()) {
+                    if (elect_one()) {
                         if (is_x)
                             tma_tile<CTAS>(sa + s * L::a_bytes, &maps.h, &full[s], full_bar + 8 * s, c, row0);
                         else
@@ -332,6 +309,7 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                 return CTAS == 2 ? mbar_test_wait_cluster(&full[i], phase) : mbar_test_wait(&full[i], phase);
             };
             bool ready = false;
+            int piece = 0;  // first column of the next adapter step's piece of the pair
             int acc = 0;
             uint32_t acc_ph = 0;
             bool ok = true;
@@ -351,7 +329,13 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                         break;
                     }
                     tc_fence_after();
-                    last = last_step[s] != 0;
+                    const int kind = step_kind[s];
+                    last = kind & kLast;
+                    uint32_t off[4 * CTAS] = {};
+                    if (kind & kMasked) {
+#pragma unroll
+                        for (int j = 0; j < 4 * CTAS; ++j) off[j] = step_off[8 * s + j];
+                    }
                     const uint64_t ad = a_desc + static_cast<uint32_t>(s * (L::a_bytes >> 4));
                     const uint64_t bd = b_desc + static_cast<uint32_t>(s * (L::b_bytes >> 4));
                     const int now = s;
@@ -360,11 +344,23 @@ routed_tile_kernel(const __grid_constant__ TileMaps maps, const RoutedProduct p,
                         ph ^= 1u;
                     }
                     ready = probe_full(s, ph);
+                    if (kind & kMasked) {
+                        // The last piece of a pair may be short of 64 columns.
+                        const int deep = min(BK, 2 * p.rank - piece);
+                        piece = piece + BK < 2 * p.rank ? piece + BK : 0;
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk) {
-                        if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
-                        else tc_mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
-                        accumulate = 1;
+                        for (int kk = 0; kk < BK / 16; ++kk) {
+                            if (16 * kk >= deep) break;
+                            if constexpr (CTAS == 2) tc_mma_f16_pair_lanes(d, ad + 2 * kk, bd + 2 * kk, idesc, off);
+                            else tc_mma_f16_lanes(d, ad + 2 * kk, bd + 2 * kk, idesc, off);
+                        }
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < BK / 16; ++kk) {
+                            if constexpr (CTAS == 2) tc_mma_f16_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
+                            else tc_mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, accumulate);
+                            accumulate = 1;
+                        }
                     }
                     if constexpr (CTAS == 2) tc_commit_both(&empty[now]);
                     else tc_commit(&empty[now]);
@@ -521,11 +517,10 @@ void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStre
         encode_tensor_map_2d(&maps.y, f16, p.y, p.n, p.rows, p.ldy * 2, 64, 32, sw);
     else
         encode_tensor_map_2d(&maps.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, p.y, p.n, p.rows, p.ldy * 4, 32, 32, sw);
-    maps.h = maps.h_rows = maps.x;
+    maps.h = maps.x;
     maps.b = maps.w;
     if (p.ids) {
         encode_tensor_map_2d(&maps.h, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, BM, sw);
-        encode_tensor_map_2d(&maps.h_rows, f16, p.h2, 2 * p.rank, p.rows, 4 * p.rank, BK, 1, sw);
         encode_tensor_map_2d(&maps.b, f16, p.b2, 2 * p.rank, static_cast<uint64_t>(p.adapter_count) * p.n, 4 * p.rank,
                              BK, BN / CTAS, sw);
     }

@@ -574,6 +574,30 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t tmem_d, uint64_t adesc,
         : "memory");
 }
 
+// tc_mma_f16 that leaves the accumulator lanes whose bits are set in `off` (lane
+// 32 w + b: bit b of off[w]) as they are.
+__device__ __forceinline__ void tc_mma_f16_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 const uint32_t (&off)[4]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+        : "memory");
+}
+// The same for a pair: words 0-3 the even CTA's lanes, 4-7 the odd one's.
+__device__ __forceinline__ void tc_mma_f16_pair_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                      const uint32_t (&off)[8]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}" ::"r"(
+            tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+        "r"(off[5]), "r"(off[6]), "r"(off[7])
+        : "memory");
+}
+
 // Arrive on the mbarrier at `bar_cluster_addr` (either CTA of the pair) once
 // every pair MMA issued so far by this thread is complete.
 __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster_addr) {
