@@ -7,14 +7,18 @@
 // dot product does not care about the order of its depth, a lane's fragment takes
 // eight consecutive columns (one 16-byte load of x, one of A_a, the same columns),
 // which serve two instructions, and the four lanes of a row read 64 bytes together.
-// A block takes 32 rows, RANK of the rank at a time (block layer z the z-th, z +
-// gridDim.z-th ... such) and one adapter of the several its rows may name (block
-// column y likewise, in rising order); its warps split the depth and add their sums
-// in shared memory in warp order.  Few rows are a chain of latencies: 16 warps, 16 of
-// the rank a block (16 rows with an adapter each, k = 1024: 12.0 -> 11.4 us with the
-// product).  Many rows are throughput: 8 warps, 32 of the rank, three blocks an SM
-// (5184 rows, rank 64: 76 us the other way round against 70).  The pair of a row
-// without adapter is not written, as nothing reads it.
+// A window of rows is cut into tasks of up to 32 rows of one adapter, in rising
+// order of the adapters; a block takes every gridDim.y-th task of a window, RANK of
+// the rank at a time (block layer z the z-th, z + gridDim.z-th ... such).  Its warps
+// split the depth and add their sums in shared memory in warp order.  (Tasks from
+// windows of 32 rows read A_a once for every few rows of a mixed batch: 33 us for 4000
+// rows of 24 adapters, rank 16, 70 us for 2000, rank 128, from windows of 256 24 and
+// 35.)  Few rows are a chain of latencies, which a larger window only lengthens (16
+// rows: 11.1 us with the product, 12.0 from 256): windows of 32, and up to 64 rows 16
+// warps, 16 of the rank a block.  Many rows are throughput: 8 warps, 32 of the rank,
+// two blocks an SM (5184 rows, rank 64: 76 us with the product the other way round
+// against 70).
+// The pair of a row without adapter is not written, as nothing reads it.
 #include <algorithm>
 
 #include "samq_internal.hpp"
@@ -22,7 +26,7 @@
 namespace samq {
 namespace {
 
-constexpr int kRows = 32;
+constexpr int kRows = 32;  // of a task
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -37,38 +41,67 @@ __device__ __forceinline__ uint4 load16(const __half* p, bool in) {
     return in ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
 
-template <int WARPS, int RANK>
+template <int WARPS, int RANK, int WINDOW>
 __global__ void __launch_bounds__(32 * WARPS)
 adapter_down_kernel(const RoutedProduct p, const __half* __restrict__ a_all, const float* __restrict__ scales,
                     const int* __restrict__ ranks, __half* __restrict__ h2, DeviceStatus* status) {
     __shared__ float part[WARPS][kRows][RANK + 1];
+    __shared__ int lists[WARPS][kRows];  // every warp's copy of the task's rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row0 = blockIdx.x * kRows;
+    const int row0 = blockIdx.x * WINDOW;
     pdl_wait();
     pdl_trigger();
-    const int rows = min(kRows, static_cast<int>(p.rows) - row0);
-    int id = lane < rows ? __ldg(p.ids + row0 + lane) : -1;
-    if (id >= p.adapter_count) id = -1;
+    int id[WINDOW / 32];  // of rows row0 + 32 j + lane
+#pragma unroll
+    for (int j = 0; j < WINDOW / 32; ++j) {
+        const int64_t row = row0 + 32 * j + lane;
+        id[j] = row < p.rows ? __ldg(p.ids + row) : -1;
+        if (id[j] >= p.adapter_count) id[j] = -1;
+    }
     const int q = lane & 3, g = lane >> 2;  // 8-column group, row of the fragment
-    int last = -1;
-    for (int index = 0;; ++index) {
-        // The next larger adapter of these rows.
-        const int a = __reduce_min_sync(0xffffffffu, id > last ? id : p.adapter_count);
-        if (a >= p.adapter_count) break;
-        last = a;
-        if (index % static_cast<int>(gridDim.y) != static_cast<int>(blockIdx.y)) continue;
+    int* list = lists[warp];
+    int a = -1, found = 0, start = 0;  // the adapter, its rows in the window, the first of the next task
+    for (int task = 0;; ++task) {
+        if (start >= found) {
+            // The next larger adapter of these rows.
+            int next = p.adapter_count;
+#pragma unroll
+            for (int j = 0; j < WINDOW / 32; ++j)
+                if (id[j] > a) next = min(next, id[j]);
+            a = __reduce_min_sync(0xffffffffu, next);
+            if (a >= p.adapter_count) break;
+            found = start = 0;
+#pragma unroll
+            for (int j = 0; j < WINDOW / 32; ++j) found += __popc(__ballot_sync(0xffffffffu, id[j] == a));
+        }
+        const int first = start;
+        start += kRows;
+        if (task % static_cast<int>(gridDim.y) != static_cast<int>(blockIdx.y)) continue;
+        const int count = min(kRows, found - first);
         const int used = __ldg(ranks + a);
         const float scale = __ldg(scales + a);
-        const unsigned members = __ballot_sync(0xffffffffu, id == a);
+        __syncthreads();  // the previous task's lists and sums have been read
+        int before = 0;
+#pragma unroll
+        for (int j = 0; j < WINDOW / 32; ++j) {
+            const unsigned in = __ballot_sync(0xffffffffu, id[j] == a);
+            const int at = before + __popc(in & ((1u << lane) - 1u)) - first;
+            if (id[j] == a && at >= 0 && at < kRows) list[at] = row0 + 32 * j + lane;
+            before += __popc(in);
+        }
+        __syncwarp();
+        const __half* xr[4];  // the fragment's rows g + 8 i
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            xr[i] = g + 8 * i < count ? p.x + static_cast<int64_t>(list[g + 8 * i]) * p.ldx + 8 * q : nullptr;
         for (int c0 = static_cast<int>(blockIdx.z) * RANK; c0 < p.rank; c0 += static_cast<int>(gridDim.z) * RANK) {
             float acc[2][RANK / 8][4] = {};
             if (c0 < used) {
                 const __half* aa = a_all + (static_cast<int64_t>(a) * p.rank + c0 + g) * p.k + 8 * q;
-                const __half* xr = p.x + static_cast<int64_t>(row0 + g) * p.ldx + 8 * q;
                 for (int k = 32 * warp; k < p.k; k += 32 * WARPS) {
                     uint4 x[4], b[RANK / 8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = load16(xr + 8 * i * p.ldx + k, (members >> (g + 8 * i)) & 1u);
+                    for (int i = 0; i < 4; ++i) x[i] = load16(xr[i] + k, xr[i] != nullptr);
 #pragma unroll
                     for (int i = 0; i < RANK / 8; ++i)
                         b[i] = load16(aa + static_cast<int64_t>(8 * i) * p.k + k, c0 + 8 * i < used);
@@ -93,12 +126,12 @@ adapter_down_kernel(const RoutedProduct p, const __half* __restrict__ a_all, con
             for (int i = threadIdx.x; i < kRows * RANK; i += 32 * WARPS) {
                 const int r = i / RANK, c = i % RANK;
                 float v = 0.0f;
-                if (((members >> r) & 1u) && c0 + c < p.rank) {
+                if (r < count && c0 + c < p.rank) {
 #pragma unroll
                     for (int w = 0; w < WARPS; ++w) v += part[w][r][c];
                     v = c0 + c < used ? v * scale : 0.0f;
                     const __half hi = __float2half_rn(v);
-                    __half* out = h2 + static_cast<int64_t>(row0 + r) * 2 * p.rank + c0 + c;
+                    __half* out = h2 + static_cast<int64_t>(list[r]) * 2 * p.rank + c0 + c;
                     out[0] = hi;
                     out[p.rank] = __float2half_rn(v - __half2float(hi));
                 }
@@ -112,19 +145,20 @@ adapter_down_kernel(const RoutedProduct p, const __half* __restrict__ a_all, con
 
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& ad, __half* h2, DeviceState& state,
                          cudaStream_t stream) {
-    const int tiles = static_cast<int>((p.rows + kRows - 1) / kRows);
-    // Few rows may name an adapter each: a block apiece.  Many rows fill the GPU by themselves.
-    const bool few = p.rows <= 64;
-    const int columns = std::max(1, std::min({ad.count, kRows, 4 * state.sm_count / tiles}));
     const __half* a = ad.a;
     const float* scale = ad.scale;
     const int* ranks = ad.ranks;
-    if (few)
-        launch_pdl(adapter_down_kernel<16, 16>, dim3(tiles, columns, p.rank / 16), dim3(512), 0, stream,
-                   "adapter_down_kernel launch", p, a, scale, ranks, h2, state.status);
-    else
-        launch_pdl(adapter_down_kernel<8, 32>, dim3(tiles, columns), dim3(256), 0, stream,
-                   "adapter_down_kernel launch", p, a, scale, ranks, h2, state.status);
+    auto run = [&](auto kernel, int threads, int window, int layers) {
+        const int windows = static_cast<int>((p.rows + window - 1) / window);
+        // Blocks of a window: as many as it may have tasks, while they fill the GPU four times at most.
+        const int most = std::min({window / kRows + ad.count, window, static_cast<int>(p.rows)});
+        const int columns = std::max(1, std::min(most, 4 * state.sm_count / windows));
+        launch_pdl(kernel, dim3(windows, columns, layers), dim3(threads), 0, stream, "adapter_down_kernel launch", p, a,
+                   scale, ranks, h2, state.status);
+    };
+    if (p.rows <= 64) run(adapter_down_kernel<16, 16, 32>, 512, 32, p.rank / 16);
+    else if (p.rows <= 256) run(adapter_down_kernel<8, 32, 32>, 256, 32, 1);
+    else run(adapter_down_kernel<8, 32, 256>, 256, 256, 1);
 }
 
 }  // namespace samq
