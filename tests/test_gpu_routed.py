@@ -126,7 +126,8 @@ def run_route(samq, logits, top_k, normalize, ld=None, workspace=True):
     (0, 8, 2, 0.0, True, None), (1, 1, 1, 0.0, True, None), (1, 8, 2, 0.0, False, 9), (31, 7, 7, 0.3, True, None),
     (64, 64, 6, 0.0, True, None), (65, 64, 6, 0.9, False, 67), (300, 100, 8, 0.5, True, None),
     (1000, 129, 3, 0.0, False, None), (700, 257, 32, 0.2, True, 300), (50, 1000, 32, 0.97, True, None),
-    (5000, 33, 4, 0.1, False, None), (40000, 16, 2, 0.0, True, None), (9000, 3, 1, 0.99, True, None)])
+    (5000, 33, 4, 0.1, False, None), (40000, 16, 2, 0.0, True, None), (9000, 3, 1, 0.99, True, None),
+    (700, 1024, 8, 0.0, False, None), (64, 128, 32, 0.4, False, 130)])
 def test_route(samq, tokens, experts, top_k, masked, normalize, ld):
     rng = np.random.default_rng(tokens * 31 + experts)
     logits = (np.round(rng.normal(0, 1.5, (tokens, experts)) * 16) / 16).astype(np.float32)  # many ties
@@ -226,7 +227,12 @@ H, F = np.float16, np.float32
     (Q4_K, 1024, 520, [0, 0, 0], H, H, False, False, {"tail": 4}),
     (Q8_0, 64, 16, [2] * 200, H, H, False, True, {}),
     (Q8_0, 1024, 256, [1500], H, H, True, False, {"tail": 7}),
-    (Q4_K, 256, 640, [5, 1100, 64], F, H, True, True, {})])
+    (Q4_K, 256, 640, [5, 1100, 64], F, H, True, True, {}),
+    (Q8_0, 64, 40, [70, 3] * 100, H, F, False, True, {"lead": 1, "tail": 1}),   # both kernels, over 128 groups
+    (Q8_0, 32, 8, [260] * 130, F, H, True, False, {}),                          # CTA pairs, over 128 groups
+    (Q6_K, 256, 392, [9, 100, 0, 17, 64, 65], H, H, True, True, {}),
+    (Q5_K, 256, 2048, [1] * 20 + [40] * 3, H, F, False, True, {"tail": 2}),
+    (Q8_0, 160, 136, [33, 64, 31], H, F, True, False, {"pad_x": 1})])
 def test_grouped(samq, oracle, qtype, k, n, sizes, x_dtype, y_dtype, gelu, gather, extra):
     got, ref, tol = grouped_case(samq, oracle, qtype, k, n, sizes, x_dtype, y_dtype, gelu, gather, **extra)
     assert_close(got, ref, tol)
@@ -270,6 +276,29 @@ def test_grouped_bad_offsets_stay_inside(samq, oracle, offsets):
     assert (host(y)[8:] == SENTINEL).all()
     samq.check(0)
     w.close()
+
+
+@pytest.mark.parametrize("rows,ld", [(70000, 32768), (5, (1 << 29) + 8)])
+def test_grouped_offsets_beyond_32_bits(samq, oracle, rows, ld):
+    """x and y of more than 2^31 elements: the last rows are right."""
+    k, n = 32, 16
+    gguf, w64 = packed(oracle, np.random.default_rng(1), Q8_0, 2 * n, k)
+    w = samq.Weights(Q8_0, k, 2 * n, gguf)
+    x = torch.empty(rows, ld, dtype=torch.float16, device="cuda")
+    y = torch.empty(rows, ld, dtype=torch.float16, device="cuda")
+    x[:, :k] = torch.randn(rows, k, device="cuda", dtype=torch.float16)
+    y[:, :n] = SENTINEL
+    cut = rows // 2
+    samq.linear_grouped(w, 2, x, rows, ld, dev(np.array([0, cut, rows - 1], np.int32)), rows, y, ld)
+    for r in (0, cut - 1, cut, rows - 2):
+        wg = w64[:n] if r < cut else w64[n:]
+        xr = host(x[r, :k]).astype(np.float64)
+        ref, tol = finished(wg @ xr, accumulation(k, np.abs(wg) @ np.abs(xr)), False, H)
+        assert_close(host(y[r, :n]), ref, tol, r)
+    assert (host(y[rows - 1, :n]) == SENTINEL).all()
+    w.close()
+    del x, y
+    torch.cuda.empty_cache()
 
 
 def test_grouped_one_group_is_the_plain_linear(samq, oracle):
@@ -569,6 +598,59 @@ def test_mixture_of_experts_layer(samq, oracle, tokens):
     samq.check(0)
     h1.close()
     h2.close()
+
+
+FIRST_CALL_IN_A_GRAPH = """
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np
+import torch
+import samq
+from oracle import oracle as o
+samq.init(0)
+rng = np.random.default_rng(0)
+E, K, N, T, J = 4, 256, 128, {tokens}, 2
+rows = o.quantize(o.Q8_0, rng.normal(0, 0.02, (E * N, K)).astype(np.float32))
+w = samq.Weights(o.Q8_0, K, E * N, rows)
+ad = samq.Adapters(K, N, 8, 2)
+ad.set(0, rng.normal(0, 0.1, (8, K)).astype(np.float16), rng.normal(0, 0.1, (N, 8)).astype(np.float16), 1.0)
+one = samq.Weights(o.Q8_0, K, N, rows.reshape(-1)[:N * o.row_bytes(o.Q8_0, K)])
+x = torch.randn(T, K, device="cuda")
+logits = torch.randn(T, E, device="cuda")
+i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+weights, ids, off, plan, slots = torch.zeros(T, J, device="cuda"), i32(T, J), i32(E + 1), i32(T * J), i32(T, J)
+y, out, z = torch.zeros(T * J, N, device="cuda"), torch.zeros(T, N, device="cuda"), torch.zeros(T, N, device="cuda")
+who = i32(T)
+def calls():
+    samq.route(logits, T, E, E, J, weights, ids, off, plan, slots)
+    samq.linear_grouped(w, E, x, T, K, off, T * J, y, N, row_index=plan)
+    samq.combine(y, T * J, N, slots, weights, T, J, N, out, N)
+    samq.linear_adapters(one, ad, x, T, K, who, z, N)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+torch.cuda.synchronize()
+first = [t.clone() for t in (weights, ids, off, plan, slots, y, out, z)]
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(first, (weights, ids, off, plan, slots, y, out, z)))
+assert out.abs().sum() > 0 and z.abs().sum() > 0
+samq.check(0)
+print("same")
+"""
+
+
+@pytest.mark.parametrize("tokens", [5, 300])
+def test_the_first_calls_may_be_captured(tokens):
+    """In a fresh process, nothing but samq_init_v1 and the handles before the capture."""
+    import subprocess
+    import sys
+    from conftest import PACKAGE, ROOT
+    code = FIRST_CALL_IN_A_GRAPH.format(paths=[str(ROOT), str(PACKAGE)], tokens=tokens)
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
 
 
 def test_two_graphs_with_workspaces_of_their_own(samq, oracle):
