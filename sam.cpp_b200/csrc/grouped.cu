@@ -82,18 +82,20 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
 
 // Few rows stream the packets, many take the f16 tiles.  Between, a call holds
 // groups of either kind and only the device knows which: both kernels run and
-// each leaves the other's groups alone.  With a mean of 16 rows or fewer the
-// packet kernel does without the second launch (and the copy of rows taken by index
-// that the tiles need) as long as even all rows in one group would cost it no more
-// than 96M decoded weights beyond one pass, about 12 us: 777 rows over 64 experts of
-// 256 -> 2048 take 18.7 us instead of 21.8, 256 over 32 of 1024 -> 4096 34.2 instead of 35.9.
+// each leaves the other's groups alone.  From a mean of 64 rows on the tiles take
+// small groups too, which are then few (640 rows over 8 groups of 1024 -> 4096: 17.0
+// us against 25.4 with both; over 64 groups of 80 rows each 139 against 134).  With a
+// mean of 16 rows or fewer the packet kernel does without the second launch as long
+// as even all rows in one group would cost it no more than 96M decoded weights beyond
+// one pass, about 12 us: 777 rows over 64 experts of 256 -> 2048 take 18.7 us instead
+// of 21.8, 256 over 32 of 1024 -> 4096 34.2 instead of 35.9.
 // With adapters the packet kernel also takes up to 256 rows of a narrow projection,
 // whose few tiles would leave most SMs idle while it splits the depth: 250 rows of
 // 100 segments, rank 24: n = 1024 16.6 us against 21.5, n = 4096 28.6 against 20.5.
 RoutedPath routed_path(int64_t rows, int groups, int64_t n, int64_t k, bool adapted) {
     if (rows <= kRoutedFewRows) return RoutedPath::kRows;
     if (adapted && rows <= kRoutedFewAdapted && (rows + 63) / 64 * ((n + 127) / 128) <= 48) return RoutedPath::kRows;
-    if (groups == 1 || rows >= int64_t(256) * groups) return RoutedPath::kTiles;
+    if (groups == 1 || rows >= int64_t(kRoutedFewRows) * groups) return RoutedPath::kTiles;
     if (rows <= int64_t(16) * groups && rows * n / 16 * k <= int64_t(96) << 20) return RoutedPath::kRows;
     return RoutedPath::kBoth;
 }

@@ -541,10 +541,25 @@ void run_tile(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStre
     }
 }
 
+// A step of 64 columns takes a CTA pair on 256 x 256 and two single CTAs on 128 x
+// 128 each the same time, as both shapes ask L2 for 32 KB an SM and step: the shape
+// of fewer waves wins, and of equal ones the single CTA, which starts and ends
+// sooner.  Row tiles: half a tile is lost at the end of every group.  Measured, waves
+// pair : single, us pair : single: 1280 rows of 8 groups to n = 4096 2 : 4, 24.8 :
+// 30.8; to n = 1024 1 : 1, 15.6 : 13.1; 2400 to n = 1024 1 : 2, 13.3 : 16.0; one group
+// of 2000 to n = 1024 1 : 1, 12.6 : 10.3.  (256-wide single CTAs and pairs 128 or 192
+// wide were nowhere more than 3% better.)
 template <int GROUPS>
 void run_shape(const RoutedProduct& p, int min_rows, DeviceState& state, cudaStream_t stream) {
-    if (p.rows >= 256 * p.groups) run_tile<2, 256, GROUPS>(p, min_rows, state, stream);
-    else run_tile<1, 128, GROUPS>(p, min_rows, state, stream);
+    auto waves = [&](int64_t height, int64_t width, int64_t units) {
+        const int64_t rows = p.groups > 1 ? p.rows + p.groups * height / 2 : p.rows + height - 1;
+        const int64_t tiles = rows / height * ((p.n + width - 1) / width);
+        return (tiles + units - 1) / units;
+    };
+    if (waves(2 * BM, 256, state.sm_count / 2) < waves(BM, 128, state.sm_count))
+        run_tile<2, 256, GROUPS>(p, min_rows, state, stream);
+    else
+        run_tile<1, 128, GROUPS>(p, min_rows, state, stream);
 }
 
 }  // namespace
