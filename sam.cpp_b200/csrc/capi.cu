@@ -1260,8 +1260,8 @@ void routed_operand(RoutedProduct& p, const void* x, int x_type, int64_t x_rows,
         return;
     }
     __half* out = static_cast<__half*>(copy);
-    if (row_index)
-        launch_gather_rows(x, x_type, x_rows, ldx, row_index, p.rows, p.k, out, state, stream);
+    if (p.offsets)
+        launch_gather_rows(x, x_type, x_rows, ldx, row_index, p.offsets, p.groups, p.rows, p.k, out, state, stream);
     else
         launch_act_f16(static_cast<const float*>(x), p.rows, p.k, ldx, out, nullptr, state.status, stream);
     p.x = out;

@@ -11,16 +11,20 @@
 namespace samq {
 namespace {
 
-// The product's operand in plan order, f16 [rows][k]: row i is x[row_index[i]]
-// (zeros for an index outside [0, x_rows)), f32 rows staged by the Q8_1 rule on
-// the way.  A thread moves 8 columns; four neighbouring threads a 32-value block.
-// Bound by memory: 2 + 2 (f16) or 4 + 2 (f32) bytes an element.
+// The product's operand in plan order, f16 [rows][k]: row i is x[row_index ?
+// row_index[i] : i], zeros for an index outside [0, x_rows) and for a row outside
+// every group (which may hold anything: it is not read, so not reported either);
+// f32 rows are staged by the Q8_1 rule on the way.  A thread moves 8 columns; four
+// neighbouring threads a 32-value block.  Bound by memory: 2 + 2 (f16) or 4 + 2
+// (f32) bytes an element.
 template <class T, int U>
 __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ x, int64_t x_rows, int64_t ldx,
-                                                          const int* __restrict__ row_index, int64_t rows, int k,
-                                                          __half* __restrict__ out, DeviceStatus* status) {
+                                                          const int* __restrict__ row_index,
+                                                          const int* __restrict__ offsets, int groups, int64_t rows,
+                                                          int k, __half* __restrict__ out, DeviceStatus* status) {
     pdl_wait();
     pdl_trigger();
+    const int begin = __ldg(offsets), end = __ldg(offsets + groups);
     const uint32_t per_row = static_cast<uint32_t>(k / 8);
     const int64_t units = rows * per_row;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -34,7 +38,8 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ 
             const int64_t u = u0 + i * stride;
             const int64_t row = u < units ? u / per_row : 0;
             c[i] = static_cast<int>(u - row * per_row) * 8;
-            src[i] = u < units ? __ldg(row_index + row) : -1;
+            src[i] = -1;
+            if (u < units && row >= begin && row < end) src[i] = row_index ? __ldg(row_index + row) : row;
             if (src[i] >= x_rows) src[i] = -1;
         }
         constexpr int W = sizeof(T) == 2 ? 1 : 2;
@@ -63,8 +68,9 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const T* __restrict__ 
 
 }  // namespace
 
-void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index, int64_t rows,
-                        int k, __half* out, DeviceState& state, cudaStream_t stream) {
+void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index,
+                        const int* offsets, int groups, int64_t rows, int k, __half* out, DeviceState& state,
+                        cudaStream_t stream) {
     // Units per thread: several where there is work for the whole GPU all the same.
     const int64_t blocks = (rows * (k / 8) + 255) / 256;
     const bool many = blocks >= 16 * state.sm_count;
@@ -74,10 +80,12 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
     const float* xf = static_cast<const float*>(x);
     if (x_type == SAMQ_TYPE_F16)
         launch_pdl(many ? gather_rows_kernel<__half, 4> : gather_rows_kernel<__half, 1>, grid, dim3(256), 0, stream,
-                   "gather_rows_kernel launch", xh, x_rows, ldx, row_index, rows, k, out, state.status);
+                   "gather_rows_kernel launch", xh, x_rows, ldx, row_index, offsets, groups, rows, k, out,
+                   state.status);
     else
         launch_pdl(many ? gather_rows_kernel<float, 4> : gather_rows_kernel<float, 1>, grid, dim3(256), 0, stream,
-                   "gather_rows_kernel launch", xf, x_rows, ldx, row_index, rows, k, out, state.status);
+                   "gather_rows_kernel launch", xf, x_rows, ldx, row_index, offsets, groups, rows, k, out,
+                   state.status);
 }
 
 // Few rows stream the packets, many take the f16 tiles.  Between, a call holds

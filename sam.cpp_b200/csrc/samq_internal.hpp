@@ -445,9 +445,11 @@ struct RoutedProduct {
     const __half* b2 = nullptr;         // [adapter_count][n][2 * rank]
     int rank = 0, adapter_count = 0;
 };
-// x[row_index[i]] as the f16 operand [rows][k] (f32 x staged by the Q8_1 rule).
-void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index, int64_t rows,
-                        int k, __half* out, DeviceState& state, cudaStream_t stream);
+// x[row_index ? row_index[i] : i] as the f16 operand [rows][k] of the rows offsets[0] .. offsets[groups] - 1,
+// zeros in the others (f32 x staged by the Q8_1 rule).
+void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, const int* row_index,
+                        const int* offsets, int groups, int64_t rows, int k, __half* out, DeviceState& state,
+                        cudaStream_t stream);
 // adapters.cu: h2 = the hi | lo pair of scale_a A_a x.
 void launch_adapter_down(const RoutedProduct& p, const samq_adapters& adapters, __half* h2, DeviceState& state,
                          cudaStream_t stream);

@@ -265,6 +265,28 @@ def test_grouped_reports_unusable_f32_activations(samq, oracle):
     w.close()
 
 
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("indexed", [False, True])
+def test_grouped_does_not_look_at_rows_outside_the_groups(samq, oracle, rows, indexed):
+    """Unusable f32 values before and behind the plan (a padded batch) are neither read nor reported."""
+    gguf, w64 = packed(oracle, np.random.default_rng(0), Q8_0, 2 * 32, 64)
+    w = samq.Weights(Q8_0, 64, 64, gguf)
+    x = torch.full((rows, 64), float("nan"), device="cuda")
+    x[3:rows - 4] = torch.randn(rows - 7, 64, device="cuda")
+    y = torch.full((rows, 32), SENTINEL, device="cuda")
+    off = np.array([3, rows // 2, rows - 4], np.int32)
+    index = dev(np.arange(rows, dtype=np.int32)) if indexed else None
+    samq.linear_grouped(w, 2, x, rows, 64, dev(off), rows, y, 32, row_index=index)
+    samq.check(0)
+    xo = operand64(oracle, host(x)[3:rows - 4])
+    got = host(y)
+    assert (got[:3] == SENTINEL).all() and (got[rows - 4:] == SENTINEL).all()
+    ref = np.stack([(w64[:32] if i + 3 < off[1] else w64[32:]) @ xo[i] for i in range(len(xo))])
+    mag = np.stack([np.abs(w64[:32] if i + 3 < off[1] else w64[32:]) @ np.abs(xo[i]) for i in range(len(xo))])
+    assert_close(got[3:rows - 4], ref, accumulation(64, mag) + 2.0 ** -24 * np.abs(ref))
+    w.close()
+
+
 @pytest.mark.parametrize("offsets", [[-5, 2, 99], [4, 1, 6], [0, 1 << 30, 3], [9, 9, 9]])
 def test_grouped_bad_offsets_stay_inside(samq, oracle, offsets):
     """Offsets out of order or out of range write no row outside [0, rows)."""
