@@ -240,12 +240,13 @@ def _addr(obj) -> int | None:
     raise TypeError(f"expected a device tensor or address, got {type(obj)!r}")
 
 
-def _stream(stream) -> int | None:
+def _stream(stream, device: int | None = None) -> int | None:
+    """The stream's address; of None, torch's current one on `device` (on the current device, if not given)."""
     if stream is None:
         try:
             import torch
             if torch.cuda.is_available():
-                return torch.cuda.current_stream().cuda_stream
+                return torch.cuda.current_stream(device).cuda_stream
         except ImportError:
             pass
         return None
@@ -766,12 +767,19 @@ def _call_on(device: int, function, *args):
         _check(status)
 
 
-def _scratch(workspace, needed: int, device: int):
-    """(tensor kept alive by the caller, address, bytes) of a workspace."""
+def _scratch(workspace, needed: int, device: int, stream):
+    """(tensor kept alive by the caller, address, bytes) of a workspace.  One taken here belongs to the call's
+    stream, so that the allocator hands it on only to what follows there."""
     if workspace is None:
         if not needed:
             return None, None, 0
-        workspace = (_torch or _load_torch()).empty(needed, dtype=_torch.uint8, device=f"cuda:{device}")
+        torch = _torch or _load_torch()
+        if stream is None:
+            workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
+        else:
+            on = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+            with torch.cuda.stream(on):
+                workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
     _same_device(device, workspace)
     return workspace, workspace.data_ptr(), workspace.nbytes
 
@@ -787,7 +795,7 @@ def route(logits, tokens: int, experts: int, ld: int, top_k: int, weights, ids, 
     _int32(ids, offsets, rows, slots)
     _float32(logits, weights)
     keep, address, size = _scratch(workspace, 0 if workspace is not None else route_workspace(tokens, experts, top_k),
-                                   device)
+                                   device, stream)
     _call_on(device, library().samq_route_v1, logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0,
              weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), address, size,
              _stream_on(stream, device))
@@ -809,7 +817,7 @@ def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, r
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt,
                                                                             row_index is not None)
-    keep, address, size = _scratch(workspace, needed, device)
+    keep, address, size = _scratch(workspace, needed, device, stream)
     status = library().samq_linear_grouped_v1(
         w.handle, groups, x.data_ptr(), xt, x_rows, ldx, None if row_index is None else row_index.data_ptr(),
         offsets.data_ptr(), rows, None if bias is None else bias.data_ptr(), epilogue, y.data_ptr(), yt, ldy, address,
@@ -835,7 +843,8 @@ class Adapters:
     def __init__(self, k: int, n: int, max_rank: int, count: int, device: int = 0, stream=None):
         handle = ctypes.c_void_p()
         self.handle = None
-        _check(library().samq_adapters_create_v1(device, k, n, max_rank, count, _stream(stream), ctypes.byref(handle)))
+        _check(library().samq_adapters_create_v1(device, k, n, max_rank, count, _stream(stream, device),
+                                               ctypes.byref(handle)))
         self.handle = handle
         self.k, self.n, self.max_rank, self.count, self.device = k, n, max_rank, count, device
 
@@ -847,10 +856,12 @@ class Adapters:
             raise ValueError("a is [rank][k], b is [n][rank]")
         a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
         _check(library().samq_adapters_set_v1(self.handle, slot, a.shape[0], a.ctypes.data, b.ctypes.data,
-                                              F16 if a.dtype == np.float16 else F32, scale, _stream(stream)))
+                                              F16 if a.dtype == np.float16 else F32, scale,
+                                              _stream(stream, self.device)))
 
     def clear(self, slot: int, stream=None):
-        _check(library().samq_adapters_set_v1(self.handle, slot, 0, None, None, F16, 0.0, _stream(stream)))
+        _check(library().samq_adapters_set_v1(self.handle, slot, 0, None, None, F16, 0.0,
+                                              _stream(stream, self.device)))
 
     def close(self):
         if self.handle:
@@ -877,7 +888,7 @@ def linear_adapters(w: Weights, adapters: Adapters, x, m: int, ldx: int, ids, y,
     _float32(bias)
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_adapters_workspace(w, adapters, m, xt)
-    keep, address, size = _scratch(workspace, needed, device)
+    keep, address, size = _scratch(workspace, needed, device, stream)
     status = library().samq_linear_adapters_v1(
         w.handle, adapters.handle, x.data_ptr(), xt, m, ldx, ids.data_ptr(), None if bias is None else bias.data_ptr(),
         epilogue, y.data_ptr(), yt, ldy, address, size, _stream_on(stream, device))

@@ -723,6 +723,34 @@ def test_two_graphs_with_workspaces_of_their_own(samq, oracle):
     w.close()
 
 
+@pytest.mark.parametrize("as_address", [False, True])
+def test_a_workspace_taken_by_the_call_belongs_to_its_stream(samq, oracle, as_address):
+    """A call on another stream than the current one, without a workspace: what the current stream allocates and
+    fills while the call has yet to run does not touch the call's memory."""
+    rng = np.random.default_rng(12)
+    k, n, m = 256, 128, 96
+    rows, _ = packed(oracle, rng, Q8_0, n, k)
+    w = samq.Weights(Q8_0, k, n, rows)
+    x = dev(rng.normal(0, 1, (m, k)).astype(F))
+    off = dev(np.array([0, m], np.int32))
+    ref, y = torch.zeros(m, n, device="cuda"), torch.zeros(m, n, device="cuda")
+    samq.linear_grouped(w, 1, x, m, k, off, m, ref, n)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+    samq.linear_grouped(w, 1, x, m, k, off, m, y, n, stream=side.cuda_stream if as_address else side)
+    size = samq.linear_grouped_workspace(w, 1, m, m, torch.float32, indexed=False)
+    filled = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    del filled
+    assert torch.equal(y, ref)
+    samq.linear_grouped(w, 1, x, m, k, off, m, y.zero_(), n, stream=0)  # the default stream by its address
+    assert torch.equal(y, ref)
+    samq.check(0)
+    w.close()
+
+
 def test_calls_are_repeatable(samq, oracle):
     """The same call twice gives the same bits (no order of arrival decides a sum)."""
     for sizes in ([1, 3, 0, 2], [70, 3, 200, 1]):
