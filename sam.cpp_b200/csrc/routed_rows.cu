@@ -41,6 +41,15 @@
 // for 75 MB of packets, 2.5 TB/s, 34 us with the rows' copy.  From a cold cache 37 us
 // with the issue slots 52% busy (4.8 instructions a weight with the epilogue) and the
 // HBM 29%: the decoders bound it, not the packet stream.
+// A decoder set takes every kSets-th packet copy of a ring that carries the adapters'
+// copies too, so it has not seen the earlier phases of the barrier it waits on, and
+// a phase's parity alone cannot tell it from the one two before.  The packet
+// producer has: it counts a copy as announced once it has found the stage free of
+// the one before, and a set waits on a stage's barrier only after its own copy's
+// announcement (a word of shared memory, read once for every few copies).  The
+// barrier is then in that copy's phase, and cannot leave it before the set has
+// decoded it.  (Waiting through every phase instead would not do: the phases of the
+// other sets' copies may be gone by two when a set comes to them.)
 // Every wait is bounded.  No load uses multicast.
 #include <algorithm>
 #include <climits>
@@ -228,6 +237,35 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// Copies announced by the packet producer (a count in this CTA's shared memory).
+__device__ __forceinline__ void announce(int* count, int copies) {
+    asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(count)), "r"(copies) : "memory");
+}
+__device__ __forceinline__ int announced(const int* count) {
+    int copies;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(copies) : "r"(smem_u32(count)) : "memory");
+    return copies;
+}
+// Bounded wait until more than `copy` copies are announced, returning their number;
+// at most `copy` when the wait is abandoned.
+__device__ __forceinline__ int wait_announced(const int* count, int copy, DeviceStatus* status, uint32_t site) {
+    int copies = announced(count);
+    if (copies > copy) return copies;
+    const uint64_t start = global_timer_ns();
+    for (uint32_t spin = 1;; ++spin) {
+        copies = announced(count);
+        if (copies > copy) return copies;
+        __nanosleep(32);
+        if ((spin & 15u) == 0 && global_timer_ns() - start > kWaitTimeoutNs) {
+            if (status) {
+                atomicOr(&status->flags, kStatusTimeout);
+                atomicExch(&status->timeout_site, site);
+            }
+            return copies;
+        }
+    }
+}
+
 __device__ __forceinline__ int clamp_row(int v, int64_t rows) {
     return v < 0 ? 0 : v > rows ? static_cast<int>(rows) : v;
 }
@@ -290,7 +328,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* part_free = part_full + 1;  // every CTA has added up what it was sent
     uint64_t* drain = part_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    static_assert((2 * kStages + 2 * kSlots + 4 + 3) * 8 + 4 <= 512, "barrier space");
+    int* s_announced = reinterpret_cast<int*>(tmem_slot + 1);
+    static_assert((2 * kStages + 2 * kSlots + 4 + 3) * 8 + 8 <= 512, "barrier space");
+    static_assert(kSlots % kSets == 0, "a set follows every phase of the slots it fills");
     int* s_begin = reinterpret_cast<int*>(smem + L::table_off);
     int* s_end = s_begin + kMaxGroups;
     int* s_first = s_end + kMaxGroups;
@@ -323,6 +363,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         mbar_init(part_full, 4 * split);
         mbar_init(part_free, 4 * split);
         mbar_init(drain, 1);
+        *s_announced = kStages;  // the first copies find their stages free
         fence_barrier_init();
         tma_prefetch_desc(&map_x);
     }
@@ -412,8 +453,9 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     const int left = min(chunks - step0 * kDepth, steps * kDepth);
                     const uint8_t* from =
                         p.packets + (static_cast<int64_t>(u.tile) * chunks + step0 * kDepth) * L::packet;
-                    for (int c = 0; c < left; c += kDepth) {
+                    for (int c = 0, copy = before; c < left; c += kDepth) {
                         if (!(ok = mbar_wait(&empty[s], ph ^ 1u, status, 71))) break;
+                        if (++copy > kStages) announce(s_announced, copy);
                         const int bytes = min(kDepth, left - c) * L::packet;
                         mbar_arrive_expect_tx(&full[s], bytes);
                         bulk_load_1d(sraw + s * L::raw_stage, from, bytes, &full[s]);
@@ -579,6 +621,7 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         const uint32_t magic = 0x64006400u + threadIdx.z;  // the compiler does not know that threadIdx.z is 0
         int done = 0;    // packet steps before this unit
         int copies = 0;  // copies of either kind before this unit
+        int known = kStages;  // copies known to be announced
         bool ok = true;
         for (int unit = cluster; unit < units && ok; unit += clusters) {
             int i = set - done % kSets;
@@ -586,9 +629,10 @@ routed_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             for (; i < steps; i += kSets) {
                 const int copy = copies + i, s = copy % kStages;
                 const int step = done + i, slot = step % kSlots;
-                ok = __all_sync(0xffffffffu,
-                                mbar_wait(&full[s], static_cast<uint32_t>(copy / kStages) & 1u, status, 77) &&
-                                    mbar_wait(&a_empty[slot], (static_cast<uint32_t>(step / kSlots) & 1u) ^ 1u, status, 78));
+                if (!mbar_wait(&a_empty[slot], (static_cast<uint32_t>(step / kSlots) & 1u) ^ 1u, status, 78)) ok = false;
+                else if (copy >= known && (known = wait_announced(s_announced, copy, status, 75)) <= copy) ok = false;
+                else ok = mbar_wait(&full[s], static_cast<uint32_t>(copy / kStages) & 1u, status, 77);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 const int here = min(kDepth, chunks - (step0 + i) * kDepth);

@@ -761,3 +761,40 @@ def test_calls_are_repeatable(samq, oracle):
         a = adapters_case(samq, oracle, Q4_K, 1024, 264, m, 16, 5, H, F, False)[0]
         b = adapters_case(samq, oracle, Q4_K, 1024, 264, m, 16, 5, H, F, False)[0]
         np.testing.assert_array_equal(a, b)
+
+
+# ---- several units of work a CTA -------------------------------------------------------
+# The packet kernel's CTAs are one an SM; beyond 148 weight row tiles (groups x n / 128) each works through several, so
+# that its rings of copies wrap around from one to the next.
+
+@pytest.mark.parametrize("qtype,k,n,m,rank,count,x_dtype,y_dtype,gelu,extra", [
+    (Q4_K, 1024, 19072, 16, 16, 16, H, F, False, {"ids": list(range(16))}),
+    (Q8_0, 1024, 40000, 64, 16, 40, H, H, False, {}),
+    (Q5_K, 512, 28680, 31, 128, 12, H, F, False, {}),
+    (Q6_K, 768, 19200, 64, 128, 10, F, F, False, {}),
+    (Q4_K, 256, 32000, 33, 8, 33, H, F, False, {"ids": list(range(33))}),
+    (Q8_0, 96, 40008, 9, 4, 9, F, H, False, {"ids": list(range(9))}),
+    (Q6_K, 1024, 19072, 5, 16, 3, H, F, False, {"bias": False}),
+    (Q5_K, 512, 19072, 32, 16, 32, H, F, True, {"ids": list(range(32))})])
+def test_adapters_of_wide_projections(samq, oracle, qtype, k, n, m, rank, count, x_dtype, y_dtype, gelu, extra):
+    got, ref, tol = adapters_case(samq, oracle, qtype, k, n, m, rank, count, x_dtype, y_dtype, gelu, **extra)
+    assert_close(got, ref, tol)
+    again = adapters_case(samq, oracle, qtype, k, n, m, rank, count, x_dtype, y_dtype, gelu, **extra)[0]
+    np.testing.assert_array_equal(got, again)
+    samq.check(0)
+
+
+@pytest.mark.parametrize("qtype,k,n,sizes,x_dtype", [
+    (Q8_0, 1024, 2504, [9, 16, 1, 7] * 4, H), (Q6_K, 1024, 2504, [16, 1, 0, 12] * 5, F),     # 16 rows at a time
+    (Q4_K, 1024, 2504, [20, 32, 17] * 4, H), (Q5_K, 512, 2504, [32, 30, 29] * 4, F),         # 32
+    (Q6_K, 2048, 2504, [18, 25, 32] * 4, H), (Q8_0, 1056, 2504, [31, 17, 26] * 4, F),
+    (Q8_0, 1024, 2504, [64, 40, 50, 33] * 3, H), (Q4_K, 1024, 2504, [60, 35, 64, 50] * 3, F),  # 64
+    (Q5_K, 2048, 2504, [64, 64, 33, 48] * 3, H), (Q6_K, 1024, 2504, [36, 64, 41, 64] * 3, F),
+    (Q8_0, 1024, 40008, [64], H), (Q5_K, 512, 40008, [33], F), (Q4_K, 256, 40008, [1], H)])
+def test_grouped_of_many_units(samq, oracle, qtype, k, n, sizes, x_dtype):
+    got, ref, tol = grouped_case(samq, oracle, qtype, k, n, sizes, x_dtype, F, False, False)
+    assert_close(got, ref, tol)
+    for _ in range(2):
+        again = grouped_case(samq, oracle, qtype, k, n, sizes, x_dtype, F, False, False)[0]
+        np.testing.assert_array_equal(got, again)
+    samq.check(0)
