@@ -1215,6 +1215,7 @@ samq_status samq_neck_forward_v1(const samq_neck_v1* neck, const float* x, int g
 namespace {
 
 constexpr int64_t kMaxRoutedRows = int64_t(1) << 24;
+constexpr int64_t kMaxRouteTokens = int64_t(1) << 20;
 constexpr int kMaxGroups = 1024;
 constexpr int kMaxTopK = 32;
 constexpr int kMaxAdapterRank = 128;
@@ -1300,7 +1301,8 @@ bool host_f16(const void* src, int type, size_t count, __half* dst) {
 }  // namespace
 
 size_t samq_route_workspace_v1(int64_t tokens, int experts, int top_k) {
-    if (tokens < 0 || experts <= 0 || top_k <= 0) return 0;
+    if (tokens < 0 || tokens > kMaxRouteTokens || experts < 1 || experts > kMaxGroups) return 0;
+    if (top_k < 1 || top_k > kMaxTopK || top_k > experts) return 0;
     return route_workspace_bytes(tokens, experts, top_k);
 }
 
@@ -1308,7 +1310,7 @@ samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int6
                           float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots,
                           void* workspace, size_t workspace_bytes, void* stream_ptr) {
     return guarded([&] {
-        require(tokens >= 0 && tokens <= (int64_t(1) << 20), "token count out of range");
+        require(tokens >= 0 && tokens <= kMaxRouteTokens, "token count out of range");
         require(experts >= 1 && experts <= kMaxGroups, "expert count out of range");
         require(top_k >= 1 && top_k <= kMaxTopK && top_k <= experts, "top_k must lie in [1, min(32, experts)]");
         require(ld >= experts && ld <= (int64_t(1) << 32), "logit row stride must be >= experts");

@@ -102,3 +102,23 @@ def test_binding_refuses_other_tensors(samq):
         samq._element(torch.bfloat16)
     assert samq._element(torch.float16) == samq.F16 and samq._element(torch.float32) == samq.F32
     assert samq._element(samq.F32) == samq.F32
+
+
+ROUTE_SIZE_OF_REFUSED = """
+import sys
+sys.path.insert(0, {path!r})
+import samq
+for tokens, experts, top_k in [(100, 64, 50000), (1 << 20, 64, 1 << 30), (100, 8, 9), (100, 64, 33), (100, 1025, 2),
+                               ((1 << 20) + 1, 64, 2), (1 << 62, 64, 2), (100, 1 << 30, 32)]:
+    assert samq.route_workspace(tokens, experts, top_k) == 0, (tokens, experts, top_k)
+print("zero")
+"""
+
+
+def test_route_workspace_of_refused_arguments():
+    """Arguments samq_route_v1 refuses need no workspace; the question ends in no division by zero (in a process of its
+    own, which one would end)."""
+    import sys
+    run = subprocess.run([sys.executable, "-c", ROUTE_SIZE_OF_REFUSED.format(path=str(PACKAGE))], capture_output=True,
+                         text=True, timeout=240)
+    assert run.returncode == 0 and "zero" in run.stdout, (run.returncode, run.stderr[-2000:])
