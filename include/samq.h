@@ -566,7 +566,10 @@ samq_status samq_neck_forward_v1(const samq_neck_v1* neck, const float* x, int g
  * f32 activations are staged by the Q8_1 rule of samq_stage_f16_v1 (into the
  * workspace), f16 activations are the operand itself, as in
  * samq_linear_f16_v1.  The weight operand is the decoded packed weight rounded
- * to f16 whatever the row count; products accumulate in f32; f16 outputs are
+ * to f16 whatever the row count; products accumulate in f32 on the tensor
+ * cores, which truncate: each 16 columns of depth may take up to 2^-23 of the
+ * running magnitude toward zero, so the error grows with k (5.6e-6 of the
+ * output's norm at k = 4736; no entry splits the depth).  f16 outputs are
  * rounded once (values beyond f16's range become infinities).
  *
  * These calls keep no memory of the library between them: what they need is
@@ -643,10 +646,14 @@ samq_status samq_adapters_destroy_v1(samq_adapters* adapters);
 
 /* The shared projection with every row's own adapter:
  *   y[i] = act(W x[i] + bias + scale_a B_a (A_a x[i])), a = ids[i],
- * for m rows; an ids[i] outside [0, count) is a row without adapter.
- * scale_a A_a x[i] is kept to f32's precision as a pair of f16 values and
- * must lie within the f16 operand range (else SAMQ_ERR_RANGE from
- * samq_check_v1).  m <= 2^24; strides, alignment and types as above. */
+ * for m rows; an ids[i] outside [0, count) is a row without adapter.  x[i] is
+ * the operand in both products: f32 activations enter A_a x[i] as staged by
+ * the Q8_1 rule too (8 bits a value); give f16 activations where that is too
+ * coarse for the adapters.  h = scale_a A_a x[i] is a sum in f32 kept as a
+ * pair of f16 values, to 2^-22 |h| + 2^-25: f32's level for |h| from 2^-3 on,
+ * an absolute 2^-25 below (a relative 3e-3 at |h| = 1e-5).  It must lie within
+ * the f16 operand range (else SAMQ_ERR_RANGE from samq_check_v1).  m <= 2^24;
+ * strides, alignment and types as above. */
 size_t samq_linear_adapters_workspace_v1(const samq_weights* weights, const samq_adapters* adapters, int64_t m,
                                          int x_type);
 samq_status samq_linear_adapters_v1(const samq_weights* weights, const samq_adapters* adapters, const void* x,

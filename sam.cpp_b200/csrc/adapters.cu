@@ -1,6 +1,10 @@
 // adapters.cu -- the down product of low-rank adapters: for every row i with
 // adapter a = ids[i], h_i = scale_a A_a x_i (rank values, f32), stored as the f16
 // pair hi | lo that routed_tile.cu multiplies as depth and routed_rows.cu adds up.
+// x is the projection's operand (of f32 activations the staged one: one operand to
+// read, and it is there).  The pair has h to 2^-22 |h| + 2^-25, as lo is subnormal
+// below |h| = 2^-3; a scale of its own would have to be taken back in B, which has
+// no bits to spare.
 //
 // Work is rank / n of the projection's, so this is a latency and L2 problem, not
 // a tensor one: mma.sync m16n8k16 straight from global memory, no staging.  As a

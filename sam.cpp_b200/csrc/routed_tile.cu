@@ -7,8 +7,8 @@
 //   delta_i = B_a h_i, h_i = scale_a A_a x_i (a = ids[i]),
 //   D += [hi(H) | lo(H)] . [B_a | B_a]^T for every adapter a with rows in the tile,
 // on the accumulator rows i with ids[i] == a alone: the MMA leaves the lanes of the
-// others as they are.  The pair keeps h to 2^-22, f32's level against the f16
-// rounding of B.  (Zeroing the other rows of the left factor by a TMA row gather
+// others as they are.  The pair keeps h to 2^-22 |h| + 2^-25: f32's level against the
+// f16 rounding of B, until lo becomes subnormal below |h| = 2^-3.  (Zeroing the other rows of the left factor by a TMA row gather
 // instead made such a step 1.2 us, three times a step of W.)
 //
 // x arrives in plan order: a row_index has been applied by gather_rows_kernel.

@@ -798,3 +798,26 @@ def test_grouped_of_many_units(samq, oracle, qtype, k, n, sizes, x_dtype):
         again = grouped_case(samq, oracle, qtype, k, n, sizes, x_dtype, F, False, False)[0]
         np.testing.assert_array_equal(got, again)
     samq.check(0)
+
+
+@pytest.mark.parametrize("m", [9, 400])
+@pytest.mark.parametrize("scale", [1.0, 0.1, 1e-3, 1e-5, 1e-7, 2.0 ** -27, 3000.0])
+def test_adapters_keep_the_down_product_to_the_stated_bound(samq, oracle, m, scale):
+    """Through a zero W and a B of ones the output is h = scale A x itself: within 2^-22 |h| + 2^-25 of it (the f16
+    pair), and the f32 arithmetic beside that: one rounding by the scale, truncated sums of two terms."""
+    rng = np.random.default_rng(int(m + 1e9 * scale))
+    k, r = 64, 16
+    w = samq.Weights(Q8_0, k, r, oracle.quantize(Q8_0, np.zeros((r, k), F)))
+    ad = samq.Adapters(k, r, r, 1)
+    a = np.zeros((r, k), H)
+    a[np.arange(r), rng.permutation(k)[:r]] = rng.uniform(0.5, 2, r).astype(H)  # one product of 22 bits each: exact
+    ad.set(0, a, np.eye(r, dtype=H), scale)
+    x = (rng.uniform(0.5, 4, (m, k)) * rng.choice([-1, 1], (m, k))).astype(H)
+    y = torch.empty(m, r, device="cuda")
+    samq.linear_adapters(w, ad, dev(x), m, k, dev(np.zeros(m, np.int32)), y, r)
+    samq.check(0)
+    h = float(np.float32(scale)) * (x.astype(np.float64) @ a.astype(np.float64).T)
+    off = np.abs(host(y) - h)
+    assert (off <= (2.0 ** -22 + 2.0 ** -24 + 2.0 ** -23) * np.abs(h) + 2.0 ** -25).all(), float((off / np.abs(h)).max())
+    ad.close()
+    w.close()
