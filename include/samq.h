@@ -595,7 +595,8 @@ samq_status samq_neck_forward_v1(const samq_neck_v1* neck, const float* x, int g
  *   rows    [tokens * top_k]: the token of each plan row, the rows of an
  *     expert in order of (token, choice); -1 from offsets[experts] on;
  *   slots   [tokens][top_k]: the plan row of each choice (the inverse).
- * The workspace size of arguments that the call refuses is 0. */
+ * The workspace size is 0 up to 64 tokens, and for arguments that the call
+ * refuses. */
 size_t samq_route_workspace_v1(int64_t tokens, int experts, int top_k);
 samq_status samq_route_v1(const float* logits, int64_t tokens, int experts, int64_t ld, int top_k, int normalize,
                           float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots,

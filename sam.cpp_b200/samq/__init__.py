@@ -697,24 +697,31 @@ def neck_forward(neck: Neck, x, grid_w: int, grid_h: int, outs, stream=None):
 
 # ---- routed linears ----------------------------------------------------------
 # Element types come from the torch tensors (float16 or float32); index tensors
-# are int32 on the device.  `workspace` is a uint8 tensor of at least the
+# are int32 on the device.  Arrays without a stride of their own (indices, weights
+# of choices, offsets, bias) are contiguous; rows with a stride (logits, x, y,
+# residual, out) may be a view whose rows lie that stride apart.  A tensor that holds
+# less than the sizes say is refused.  `workspace` is a uint8 tensor of at least the
 # ..._workspace() size, kept by a caller that calls often or captures a graph;
 # without one a call that needs memory takes it from torch's caching allocator.
 
 _elements = {}
-_torch = None  # torch, once a routed call has needed it (the binding itself does not)
+# torch and what a call needs of it at once, from the first routed call on (the binding itself does not need it)
+_torch = _f32 = _i32 = _current_device = _current_stream = None
 
 
 def _load_torch():
-    global _torch
+    global _torch, _f32, _i32, _current_device, _current_stream
     import torch
     _elements.update({torch.float16: F16, torch.float32: F32})
-    _torch = torch
+    _torch, _f32, _i32 = torch, torch.float32, torch.int32
+    _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     return torch
 
 
 def _element(dtype) -> int:
     """F16 / F32 of a torch dtype (or the id itself)."""
+    if dtype in _elements:
+        return _elements[dtype]
     if isinstance(dtype, int):
         return dtype
     if _torch is None:
@@ -724,44 +731,68 @@ def _element(dtype) -> int:
     return _elements[dtype]
 
 
-def _same_device(device: int | None, *tensors) -> int:
-    """The one CUDA device of the given tensors (None entries skipped), which must be `device` where that is given."""
-    for t in tensors:
-        if t is not None:
-            d = t.get_device()  # -1 off the GPU
-            if d < 0 or (device is not None and d != device):
-                raise ValueError(f"tensor on {t.device}, expected cuda:{'' if device is None else device}")
-            device = d
+def _device_of(t) -> int:
+    device = t.get_device()  # -1 off the GPU
+    if device < 0:
+        raise ValueError(f"tensor on {t.device}, expected cuda:")
     return device
 
 
 def _int32(*tensors):
-    int32 = (_torch or _load_torch()).int32
+    if _torch is None:
+        _load_torch()
     for t in tensors:
-        if t is not None and t.dtype is not int32:
+        if t is not None and t.dtype is not _i32:
             raise TypeError(f"index tensors are int32, got {t.dtype}")
 
 
-def _float32(*tensors):
-    float32 = (_torch or _load_torch()).float32
+def _array(device: int, dtype, count: int, *tensors):
+    """Contiguous tensors of at least `count` elements of `dtype` on `device` (None entries skipped)."""
     for t in tensors:
-        if t is not None and t.dtype is not float32:
-            raise TypeError(f"float32 expected, got {t.dtype}")
+        if t is None or (t.get_device() == device and t.dtype is dtype and t.numel() >= count and t.is_contiguous()):
+            continue
+        if t.get_device() != device:
+            raise ValueError(f"tensor on {t.device}, expected cuda:{device}")
+        if dtype is _i32:
+            _int32(t)
+        if t.dtype is not dtype:
+            raise TypeError(f"{dtype} expected, got {t.dtype}")
+        raise ValueError(f"a contiguous tensor of {count} elements or more expected, got {tuple(t.shape)} with strides "
+                         f"{t.stride()}")
+
+
+def _rows(device: int, t, rows: int, ld: int, width: int):
+    """A tensor on `device` with `rows` rows of `width` elements, `ld` elements apart."""
+    if t.get_device() != device:
+        raise ValueError(f"tensor on {t.device}, expected cuda:{device}")
+    need = (rows - 1) * ld + width if rows > 0 else 0
+    if t.numel() >= need and t.is_contiguous():
+        return
+    shape, stride = tuple(t.shape), t.stride()
+    reach = 1 + sum((n - 1) * step for n, step in zip(shape, stride)) if t.numel() else 0  # from first to last element
+    if reach < need or (shape and shape[-1] > 1 and stride[-1] != 1) or \
+            (len(shape) == 2 and shape[0] > 1 and stride[0] != ld):
+        raise ValueError(f"{rows} rows of {width} elements, {ld} apart, expected, got {shape} with strides {stride}")
+
+
+def _float32_rows(device: int, t, rows: int, ld: int, width: int):
+    if t.dtype is not _f32:
+        raise TypeError(f"float32 expected, got {t.dtype}")
+    _rows(device, t, rows, ld, width)
 
 
 def _stream_on(stream, device: int):
     if stream is None:
-        return (_torch or _load_torch())._C._cuda_getCurrentRawStream(device)
+        return _current_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _call_on(device: int, function, *args):
+def _call_on(device: int, function, args: tuple):
     """A call that runs on the current device, with `device` made current where it is not."""
-    torch = _torch or _load_torch()
-    if torch._C._cuda_getDevice() == device:
+    if _current_device() == device:
         status = function(*args)
     else:
-        with torch.cuda.device(device):
+        with _torch.cuda.device(device):
             status = function(*args)
     if status:
         _check(status)
@@ -773,14 +804,15 @@ def _scratch(workspace, needed: int, device: int, stream):
     if workspace is None:
         if not needed:
             return None, None, 0
-        torch = _torch or _load_torch()
+        torch = _torch
         if stream is None:
             workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
         else:
             on = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
             with torch.cuda.stream(on):
                 workspace = torch.empty(needed, dtype=torch.uint8, device=f"cuda:{device}")
-    _same_device(device, workspace)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError(f"the workspace is a contiguous tensor on cuda:{device}, got one on {workspace.device}")
     return workspace, workspace.data_ptr(), workspace.nbytes
 
 
@@ -791,14 +823,29 @@ def route_workspace(tokens: int, experts: int, top_k: int) -> int:
 def route(logits, tokens: int, experts: int, ld: int, top_k: int, weights, ids, offsets, rows, slots,
           normalize: bool = True, workspace=None, stream=None):
     """samq_route_v1: the top_k experts of every row of logits, their weights and the plan sorted by expert."""
-    device = _same_device(None, logits, weights, ids, offsets, rows, slots)
-    _int32(ids, offsets, rows, slots)
-    _float32(logits, weights)
-    keep, address, size = _scratch(workspace, 0 if workspace is not None else route_workspace(tokens, experts, top_k),
-                                   device, stream)
-    _call_on(device, library().samq_route_v1, logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0,
-             weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), address, size,
-             _stream_on(stream, device))
+    if _torch is None:
+        _load_torch()
+    device, choices = logits.get_device(), tokens * top_k
+    # The usual call in one expression, as the host's issue is what a small one takes.
+    if not (device >= 0 and logits.dtype is _f32 and logits.numel() >= tokens * ld and logits.is_contiguous() and
+            weights.get_device() == device and weights.dtype is _f32 and weights.numel() >= choices and
+            weights.is_contiguous() and ids.get_device() == device and ids.dtype is _i32 and ids.numel() >= choices and
+            ids.is_contiguous() and rows.get_device() == device and rows.dtype is _i32 and rows.numel() >= choices and
+            rows.is_contiguous() and slots.get_device() == device and slots.dtype is _i32 and
+            slots.numel() >= choices and slots.is_contiguous() and offsets.get_device() == device and
+            offsets.dtype is _i32 and offsets.numel() > experts and offsets.is_contiguous()):
+        _float32_rows(_device_of(logits), logits, tokens, ld, experts)
+        _array(device, _f32, choices, weights)
+        _array(device, _i32, choices, ids, rows, slots)
+        _array(device, _i32, experts + 1, offsets)
+    keep = address = None
+    size = 0
+    if workspace is not None or tokens > 64:  # up to 64 tokens take none
+        needed = 0 if workspace is not None else route_workspace(tokens, experts, top_k)
+        keep, address, size = _scratch(workspace, needed, device, stream)
+    _call_on(device, library().samq_route_v1, (
+        logits.data_ptr(), tokens, experts, ld, top_k, 1 if normalize else 0, weights.data_ptr(), ids.data_ptr(),
+        offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), address, size, _stream_on(stream, device)))
 
 
 def linear_grouped_workspace(w: Weights, groups: int, x_rows: int, rows: int, x_dtype, indexed: bool = True) -> int:
@@ -811,9 +858,16 @@ def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, r
                    bias=None, epilogue: int = EPILOGUE_NONE, workspace=None, stream=None):
     """samq_linear_grouped_v1: y[i] = act(W_g x[row_index[i]] + bias_g) for the rows offsets[g] .. offsets[g + 1] of
     group g; w holds the groups' matrices stacked (w.n = groups * n)."""
-    device = _same_device(w.device, x, offsets, y, row_index, bias)
-    _int32(offsets, row_index)
-    _float32(bias)
+    if _torch is None:
+        _load_torch()
+    device = w.device
+    _rows(device, x, x_rows, ldx, w.k)
+    _rows(device, y, rows, ldy, w.n // groups if groups > 0 else 0)
+    _array(device, _i32, groups + 1, offsets)
+    if row_index is not None:
+        _array(device, _i32, rows, row_index)
+    if bias is not None:
+        _array(device, _f32, w.n, bias)
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_grouped_workspace(w, groups, x_rows, rows, xt,
                                                                             row_index is not None)
@@ -829,12 +883,26 @@ def linear_grouped(w: Weights, groups: int, x, x_rows: int, ldx: int, offsets, r
 def combine(y, y_rows: int, ldy: int, slots, weights, tokens: int, top_k: int, width: int, out, ldo: int,
             residual=None, ldr: int = 0, stream=None):
     """samq_combine_v1: out[t] = residual[t] + sum_j weights[t][j] y[slots[t][j]]."""
-    device = _same_device(None, y, slots, weights, out, residual)
-    _int32(slots)
-    _float32(weights, out, residual)
-    _call_on(device, library().samq_combine_v1, y.data_ptr(), _element(y.dtype), y_rows, ldy, slots.data_ptr(),
-             weights.data_ptr(), tokens, top_k, width, None if residual is None else residual.data_ptr(), ldr,
-             out.data_ptr(), ldo, _stream_on(stream, device))
+    if _torch is None:
+        _load_torch()
+    device, choices = y.get_device(), tokens * top_k
+    # As in route().
+    if not (device >= 0 and y.numel() >= y_rows * ldy and y.is_contiguous() and slots.get_device() == device and
+            slots.dtype is _i32 and slots.numel() >= choices and slots.is_contiguous() and
+            weights.get_device() == device and weights.dtype is _f32 and weights.numel() >= choices and
+            weights.is_contiguous() and out.get_device() == device and out.dtype is _f32 and
+            out.numel() >= tokens * ldo and out.is_contiguous() and
+            (residual is None or (residual.get_device() == device and residual.dtype is _f32 and
+                                  residual.numel() >= tokens * ldr and residual.is_contiguous()))):
+        _rows(_device_of(y), y, y_rows, ldy, width)
+        _array(device, _i32, choices, slots)
+        _array(device, _f32, choices, weights)
+        _float32_rows(device, out, tokens, ldo, width)
+        if residual is not None:
+            _float32_rows(device, residual, tokens, ldr, width)
+    _call_on(device, library().samq_combine_v1, (
+        y.data_ptr(), _element(y.dtype), y_rows, ldy, slots.data_ptr(), weights.data_ptr(), tokens, top_k, width,
+        None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldo, _stream_on(stream, device)))
 
 
 class Adapters:
@@ -883,9 +951,14 @@ def linear_adapters(w: Weights, adapters: Adapters, x, m: int, ldx: int, ids, y,
                     epilogue: int = EPILOGUE_NONE, workspace=None, stream=None):
     """samq_linear_adapters_v1: y[i] = act(W x[i] + bias + scale_a B_a (A_a x[i])) with a = ids[i] (none if out of
     range)."""
-    device = _same_device(w.device, x, ids, y, bias)
-    _int32(ids)
-    _float32(bias)
+    if _torch is None:
+        _load_torch()
+    device = w.device
+    _rows(device, x, m, ldx, w.k)
+    _rows(device, y, m, ldy, w.n)
+    _array(device, _i32, m, ids)
+    if bias is not None:
+        _array(device, _f32, w.n, bias)
     xt, yt = _element(x.dtype), _element(y.dtype)
     needed = 0 if workspace is not None else linear_adapters_workspace(w, adapters, m, xt)
     keep, address, size = _scratch(workspace, needed, device, stream)

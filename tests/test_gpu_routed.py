@@ -821,3 +821,52 @@ def test_adapters_keep_the_down_product_to_the_stated_bound(samq, oracle, m, sca
     assert (off <= (2.0 ** -22 + 2.0 ** -24 + 2.0 ** -23) * np.abs(h) + 2.0 ** -25).all(), float((off / np.abs(h)).max())
     ad.close()
     w.close()
+
+
+def test_binding_refuses_what_the_sizes_do_not_fit(samq, oracle):
+    """Tensors that are too small, not contiguous, or strided otherwise than stated are refused before any launch; views
+    whose rows lie the stated stride apart are taken."""
+    t, e, j, k, n = 70, 4, 2, 64, 32
+    logits = torch.randn(t, e + 2, device="cuda")
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    route = {"logits": logits[:, 1:e + 1], "tokens": t, "experts": e, "ld": e + 2, "top_k": j,
+             "weights": torch.zeros(t, j, device="cuda"), "ids": i32(t, j), "offsets": i32(e + 1), "rows": i32(t * j),
+             "slots": i32(t, j)}
+    samq.route(**route)
+    for name, bad in (("ids", i32(j, t).t()), ("slots", i32(t - 1, j)), ("offsets", i32(e)), ("rows", i32(t * j, 2)[:, 0]),
+                      ("weights", torch.zeros(t, 2 * j, device="cuda")[:, :j]), ("logits", logits[:, 3:]),
+                      ("logits", logits[1:]), ("logits", logits.t())):
+        with pytest.raises(ValueError):
+            samq.route(**{**route, name: bad})
+    rows, _ = packed(oracle, np.random.default_rng(0), Q8_0, e * n, k)
+    w, one = samq.Weights(Q8_0, k, e * n, rows), samq.Weights(Q8_0, k, n, rows.reshape(-1)[:rows.size // e])
+    x = torch.randn(t, k + 8, device="cuda", dtype=torch.float16)
+    y = torch.zeros(t * j, n + 8, device="cuda")
+    grouped = {"w": w, "groups": e, "x": x[:, 8:], "x_rows": t, "ldx": k + 8, "offsets": route["offsets"], "rows": t * j,
+               "y": y[:, 4:], "ldy": n + 8, "row_index": route["rows"], "bias": torch.zeros(e, n, device="cuda")}
+    samq.linear_grouped(**grouped)
+    for name, bad in (("x", x[1:]), ("x", x[:, 16:]), ("y", y[:, 12:]), ("offsets", i32(e)), ("row_index", i32(t)),
+                      ("bias", torch.zeros(n, device="cuda")), ("rows", t * j + 1), ("x_rows", t + 1), ("ldx", k),
+                      ("workspace", torch.zeros(8, dtype=torch.uint8, device="cuda").expand(1 << 16, 8))):
+        with pytest.raises(ValueError):
+            samq.linear_grouped(**{**grouped, name: bad})
+    combine = {"y": y[:, 4:], "y_rows": t * j, "ldy": n + 8, "slots": route["slots"], "weights": route["weights"],
+               "tokens": t, "top_k": j, "width": n, "out": torch.zeros(t, n, device="cuda"), "ldo": n,
+               "residual": torch.zeros(t, n + 4, device="cuda")[:, :n], "ldr": n + 4}
+    samq.combine(**combine)
+    for name, bad in (("y_rows", t * j + 1), ("slots", i32(j, t).t()), ("weights", torch.zeros(t, device="cuda")),
+                      ("out", torch.zeros(t - 1, n, device="cuda")), ("ldr", n), ("tokens", t + 1)):
+        with pytest.raises(ValueError):
+            samq.combine(**{**combine, name: bad})
+    ad = samq.Adapters(k, n, 4, 2)
+    adapters = {"w": one, "adapters": ad, "x": x[:, 8:], "m": t, "ldx": k + 8, "ids": i32(t), "y": y[:, 4:],
+                "ldy": n + 8, "bias": torch.zeros(n, device="cuda")}
+    samq.linear_adapters(**adapters)
+    for name, bad in (("x", x[1:]), ("ids", i32(t - 1)), ("ids", i32(t, 2)[:, 1]), ("y", y[:t - 1]),
+                      ("bias", torch.zeros(n - 1, device="cuda")), ("ldx", k), ("m", 2 * t + 1)):
+        with pytest.raises(ValueError):
+            samq.linear_adapters(**{**adapters, name: bad})
+    samq.check(0)
+    ad.close()
+    w.close()
+    one.close()

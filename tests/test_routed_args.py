@@ -122,3 +122,35 @@ def test_route_workspace_of_refused_arguments():
     run = subprocess.run([sys.executable, "-c", ROUTE_SIZE_OF_REFUSED.format(path=str(PACKAGE))], capture_output=True,
                          text=True, timeout=240)
     assert run.returncode == 0 and "zero" in run.stdout, (run.returncode, run.stderr[-2000:])
+
+
+def test_binding_refuses_tensors_that_hold_too_little(samq):
+    """The checks behind the routed calls, on CPU tensors (device index -1)."""
+    torch = pytest.importorskip("torch")
+    samq._load_torch()
+    ids = torch.zeros(8, 4, dtype=torch.int32)
+    samq._array(-1, torch.int32, 32, ids, ids.view(-1), None)
+    samq._array(-1, torch.int32, 0, ids[:0])
+    for bad in (ids.t(), ids[:, :2], ids[:7], ids[0].expand(8, 4)):
+        with pytest.raises(ValueError, match="contiguous tensor of 32 elements"):
+            samq._array(-1, torch.int32, 32, bad)
+    with pytest.raises(TypeError, match="int32"):
+        samq._array(-1, torch.int32, 32, ids.long())
+    with pytest.raises(TypeError, match="float32"):
+        samq._array(-1, torch.float32, 32, ids)
+    with pytest.raises(ValueError, match="tensor on cpu, expected cuda:0"):
+        samq._array(0, torch.int32, 32, ids)
+
+    x = torch.zeros(10, 24)
+    for ok, rows, ld, width in ((x, 10, 24, 24), (x, 9, 24, 8), (x[:, 8:], 10, 24, 16), (x[2:, :8], 8, 24, 8),
+                                (x.view(-1), 20, 12, 12), (x[0], 1, 99, 24), (x, 0, 24, 24),
+                                (x[9:, 23:], 1, 8, 1), (x.view(2, 5, 24)[:, :, :8], 10, 24, 8), (x[:0], 0, 24, 24)):
+        samq._rows(-1, ok, rows, ld, width)
+    for bad, rows, ld, width in ((x, 11, 24, 24), (x[:, 8:], 10, 24, 17), (x[:, 20:], 10, 24, 8), (x[1:], 10, 24, 24),
+                                 (x.t(), 10, 24, 24), (x[:, :8], 10, 8, 8), (x[0].expand(10, 24), 10, 24, 24),
+                                 (x, 1 << 40, 24, 24), (x[:0], 1, 24, 24), (x, 10, 32, 24), (x[:7], 10, 24, 24),
+                                 (x[:, 20:], 10, 24, 5)):
+        with pytest.raises(ValueError, match="rows of"):
+            samq._rows(-1, bad, rows, ld, width)
+    with pytest.raises(TypeError, match="float32"):
+        samq._float32_rows(-1, x.half(), 10, 24, 24)
