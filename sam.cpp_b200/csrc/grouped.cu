@@ -91,15 +91,24 @@ void launch_gather_rows(const void* x, int x_type, int64_t x_rows, int64_t ldx, 
 // Few rows stream the packets, many take the f16 tiles.  Between, a call holds
 // groups of either kind and only the device knows which: both kernels run and
 // each leaves the other's groups alone.  From a mean of 64 rows on the tiles take
-// small groups too, which are then few (640 rows over 8 groups of 1024 -> 4096: 17.0
-// us against 25.4 with both; over 64 groups of 80 rows each 139 against 134).  With a
-// mean of 16 rows or fewer the packet kernel does without the second launch as long
-// as even all rows in one group would cost it no more than 96M decoded weights beyond
-// one pass, about 12 us: 777 rows over 64 experts of 256 -> 2048 take 18.7 us instead
-// of 21.8, 256 over 32 of 1024 -> 4096 34.2 instead of 35.9.
+// small groups too, which are then few.  Tiles : both : packets alone, us, groups of
+// equal size, 1024 -> 4096 Q4_K: 8 groups of 80 rows 18 : 20 : 28, of 64 17 : 20 : 17,
+// of 48 18 : 18 : 16; 64 groups of 80 149 : 151 : 155, of 48 146 : 92 : 87.  The rule's
+// worst case is many groups that all have just 64 rows: 64 such take 147 instead of 99
+// (the f16 expansion of every group against its packets).
+// With a mean of 16 rows or fewer the packet kernel does without the second launch as
+// long as even all rows in one group would cost it no more than 96M decoded weights
+// beyond one pass.  Packets alone : both, us, rows spread evenly and all in one group:
+// 777 over 64 of 256 -> 2048 Q6_K 18 : 21 and 17 : 14; 256 over 32 of 1024 -> 4096 Q4_K
+// 29 : 32 and 19 : 14; at the limit 384 over 32 30 : 33 and 26 : 17, 192 over 16 of
+// 2048 -> 4096 Q8_0 35 : 37 and 24 : 19.  So it gains 3 us where groups are alike and
+// loses at most 9 where they are not.
 // With adapters the packet kernel also takes up to 256 rows of a narrow projection,
-// whose few tiles would leave most SMs idle while it splits the depth: 250 rows of
-// 100 segments, rank 24: n = 1024 16.6 us against 21.5, n = 4096 28.6 against 20.5.
+// whose few tiles would leave most SMs idle while it splits the depth.  Packets :
+// tiles, us, 32 adapters of rank 24 and 4 of rank 16: 250 rows to n = 1024 17 : 23 and
+// 11 : 13, to 1536 23 : 24 and 13 : 12, to 2560 25 : 22 and 11 : 12, to 4096 29 : 22 and
+// 12 : 13; 100 rows to 2048 19 : 23 and 11 : 12, to 2560 25 : 23 and 14 : 13.  They meet
+// between 40 and 64 units of 64 rows by 128 weight rows: hence 48.
 RoutedPath routed_path(int64_t rows, int groups, int64_t n, int64_t k, bool adapted) {
     if (rows <= kRoutedFewRows) return RoutedPath::kRows;
     if (adapted && rows <= kRoutedFewAdapted && (rows + 63) / 64 * ((n + 127) / 128) <= 48) return RoutedPath::kRows;

@@ -26,21 +26,22 @@
 //                turns a row of its packets into f16 with the values of packets.cuh bit
 //                for bit and stores it to tensor memory, where the MMA takes it as its
 //                left factor.
-// Beside the decoders, who fill the issue slots, a copy costs the thread that
-// issues it about 500 cycles and a step the MMA thread 400, while a Q4_K packet
-// takes 210 cycles of HBM bandwidth: hence several packets a copy and a step, and
-// one thread per kind of copy.
-// The decoders' arithmetic, where the logic pipe at half rate is the bound: codes
+// Each copy and each step costs the one thread that issues it a round of waiting
+// beside the decoders' many warps: hence several packets a copy and a step (the case
+// below: 34.5 us with four, 36.8 with two, 43.6 with one), and one thread per kind of
+// copy.
+// The decoders' arithmetic spares the logic pipe, which runs at half rate: codes
 // two at a time become halves by or-ing them into the mantissa of 1024 where they
 // stand; the sum of such a half and -1024 as a float is exact and one operation of
 // the full-rate pipe (add.f32.f16), and pairs of weights share packed f32 operations.
 // An int8 is offset to be positive first, and f16(q d) needs a single half
-// multiplication as q d has at most 19 bits.  With floats from the mantissa of 2^23 a
-// Q4_K weight took 1.8 logic operations, this way 1.1.
-// Measured (128 rows of 32 experts, 1024 -> 4096 Q4_K, two experts a row, GELU): 30 us
-// for 75 MB of packets, 2.5 TB/s, 34 us with the rows' copy.  From a cold cache 37 us
-// with the issue slots 52% busy (4.8 instructions a weight with the epilogue) and the
-// HBM 29%: the decoders bound it, not the packet stream.
+// multiplication as q d has at most 19 bits.
+// Measured (128 rows of 32 experts, 1024 -> 4096 Q4_K, two experts a row, GELU): 29 us
+// for 75 MB of packets, 2.6 TB/s, 34.4 us with the rows' copy.  From a cold cache 38 us
+// with the issue slots 52% busy (4.9 instructions a weight with the epilogue), the
+// logic pipe 41% and the HBM 28%: no unit is full.  A quarter of the warps an SM could
+// hold is there, and the rest of the time they wait on one another's hand-overs: the
+// decoders bound it by latency, not the packet stream.
 // A decoder set takes every kSets-th packet copy of a ring that carries the adapters'
 // copies too, so it has not seen the earlier phases of the barrier it waits on, and
 // a phase's parity alone cannot tell it from the one two before.  The packet

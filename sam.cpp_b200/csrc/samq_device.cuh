@@ -57,8 +57,8 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 
 // True in one thread of a converged warp.  Branches on this rather than on a lane
 // index let the compiler keep the operands of the instructions that need uniform
-// registers (tcgen05.mma, TMA) there: 10 cycles per issued 128 x 16 x 16 MMA
-// against 46 behind `lane == 0`.
+// registers (tcgen05.mma, TMA) there: per issued 128 x 16 x 16 MMA 10 cycles against
+// 46 behind `lane == 0` with A in tensor memory, 40 against 46 from shared memory.
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
     asm volatile(
@@ -251,11 +251,6 @@ __device__ __forceinline__ float gelu_erf(float x) {
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
