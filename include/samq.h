@@ -624,7 +624,8 @@ samq_status samq_linear_grouped_v1(const samq_weights* weights, int groups, cons
  * weights[t][j] * y[slots[t][j]] in order of j, accumulated in f32.  y
  * [y_rows][ldy] of y_type; a slot outside [0, y_rows) adds nothing (its
  * weight is not read as a factor); residual f32 [tokens][ldr] or NULL (zero),
- * may be out itself; out f32 [tokens][ldo].  width % 4 == 0 (f32 y) or
+ * may be out itself with ldr == ldo; out f32 [tokens][ldo], which overlaps no
+ * other input.  width % 4 == 0 (f32 y) or
  * % 8 == 0 (f16 y), strides likewise, pointers 16-byte aligned, top_k <= 32. */
 samq_status samq_combine_v1(const void* y, int y_type, int64_t y_rows, int64_t ldy, const int32_t* slots,
                             const float* weights, int64_t tokens, int top_k, int64_t width, const float* residual,

@@ -1382,6 +1382,7 @@ samq_status samq_combine_v1(const void* y, int y_type, int64_t y_rows, int64_t l
         if (residual)
             check_rows(residual, SAMQ_TYPE_F32, width, ldr,
                        "residual must be 16-byte aligned with a row stride >= width, a multiple of 4");
+        require(residual != out || ldr == ldo, "residual and out in one place need one row stride");
         device_state(current_device());
         launch_combine(y, y_type, y_rows, ldy, slots, weights, tokens, top_k, width, residual, ldr, out, ldo,
                        static_cast<cudaStream_t>(stream_ptr));

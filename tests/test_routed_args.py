@@ -154,3 +154,9 @@ def test_binding_refuses_tensors_that_hold_too_little(samq):
             samq._rows(-1, bad, rows, ld, width)
     with pytest.raises(TypeError, match="float32"):
         samq._float32_rows(-1, x.half(), 10, 24, 24)
+
+
+def test_combine_in_place_takes_one_stride(samq):
+    """The residual in place of the sum: of another row stride, rows would be written before others have read them."""
+    refused(samq, "samq_combine_v1", changed(COMBINE, residual=P, out=P, ldr=64, ldo=128), "residual")
+    refused(samq, "samq_combine_v1", changed(COMBINE, residual=P, out=P, ldr=128, ldo=64), "residual")
